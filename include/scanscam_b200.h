@@ -439,6 +439,103 @@ int ssb_shard_map_publish_f32(const float *gate, const float *other, int64_t row
 int ssb_shard_carry_peer_f32(const ssb_peer_exchange_t *exchange, unsigned epoch, int backward, float *carry,
                              void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Selective state-space operators (the reference has none of them).
+ *
+ * Selective scan, per channel c and state n:
+ *     dt  = softplus(dt_raw + dt_bias) or dt_raw + dt_bias
+ *     h_t = exp(dt_t A[c,n]) h_{t-1} + dt_t x_t B_t[n]
+ *     y_t = sum_n C_t[n] h_t[n] + D x_t,      out = y silu(z)   (y where z is NULL)
+ * Short causal convolution, per channel, widths 2, 3, 4:
+ *     v_t = bias + sum_j w[j] x_{t-W+1+j},    out = v or silu(v)
+ *
+ * Tensors are described by views: a device pointer and strides in elements, so that slices of a
+ * projection and either layout (time adjacent, or channels adjacent) are taken as they are.
+ * Sequences: row n of the batch is sequence n, all `steps` of it or its first lengths[n]; or, with
+ * `offsets` (batch must be 1), sequence s is steps offsets[s] .. offsets[s+1] of the one row.
+ * offsets and lengths are read on the device and cut to [0, steps].  Outputs and gradients at
+ * steps that no sequence covers are zero.  Per-sequence states are dense: [sequences, C, S] float32
+ * for the scan, [sequences, C, W-1] in the tensors' type for the convolution.
+ * All arithmetic, states and sums are float32; an output is rounded once.
+ * ---------------------------------------------------------------------------------- */
+typedef enum ssb_dtype { SSB_F32 = 0, SSB_BF16 = 1, SSB_F16 = 2 } ssb_dtype_t;
+
+typedef struct ssb_view {
+    void *data;        /* NULL: absent (where the operand is optional) */
+    int64_t stride[4]; /* elements; [N, C, T]: n, c, t.  [N, G, S, T]: n, g, s, t.  [M, C]: m, c.  [M, G, S]: m, g, s */
+} ssb_view_t;
+
+typedef struct ssb_selective {
+    int dtype, softplus;                              /* ssb_dtype_t of the views */
+    int64_t batch, channels, steps, states, groups;   /* channels % groups == 0; states 1 .. 256 */
+    int64_t sequences;                                /* packed sequences, 1 at least; ignored where offsets is NULL */
+    const int32_t *offsets;                           /* [sequences + 1] or NULL */
+    const int32_t *lengths;                           /* [batch] or NULL; not together with offsets */
+    ssb_view_t x, dt, z, B, C, out;                   /* z optional; out is not read by the backward */
+    const float *A, *D, *dt_bias;                     /* [C, S] dense, [C], [C]; D and dt_bias optional */
+    const float *state;                               /* state before the first step, or NULL for zero */
+    float *state_out;                                 /* state behind the last step, or NULL */
+    float *checkpoints;                               /* forward: written for the backward, or NULL; backward: read */
+} ssb_selective_t;
+
+typedef struct ssb_selective_grads {
+    ssb_view_t gout;                  /* upstream */
+    const float *gstate_out;          /* upstream gradient of state_out, or NULL */
+    ssb_view_t gx, gdt, gz, gB, gC;   /* gz where z is given */
+    float *gA, *gD, *gdt_bias;        /* gD, gdt_bias optional */
+    float *gstate;                    /* optional */
+} ssb_selective_grads_t;
+
+/* Bytes of the checkpoints a forward writes for the backward of the same problem. */
+size_t ssb_selective_checkpoint_bytes(const ssb_selective_t *p);
+int ssb_selective_fwd(const ssb_selective_t *p, void *stream);
+size_t ssb_selective_bwd_workspace_bytes(const ssb_selective_t *p);
+int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/* One step for each of `entries` tokens on a pool of states [pool, C, S], updated in place.  Entry m
+ * works on state slots[m] (m where slots is NULL); a slot outside the pool marks an idle entry,
+ * whose output is zero.  Entries that name the same slot are consecutive tokens, in batch order. */
+typedef struct ssb_selective_step {
+    int dtype, softplus;
+    int64_t entries, channels, states, groups, pool;
+    const int32_t *slots;
+    ssb_view_t x, dt, z, B, C, out;
+    const float *A, *D, *dt_bias;
+    float *state;
+} ssb_selective_step_t;
+int ssb_selective_step(const ssb_selective_step_t *p, void *stream);
+
+typedef struct ssb_short_conv {
+    int dtype, silu, weight_f32;                  /* weight_f32: weight and bias are float32, else in `dtype` */
+    int64_t batch, channels, steps, width;
+    int64_t sequences;
+    const int32_t *offsets, *lengths;             /* offsets: channels-last views only (stride of c is 1) */
+    ssb_view_t x, out;
+    const void *weight, *bias;                    /* [C, W], [C] dense; bias optional */
+    const void *state;                            /* the window carried in, oldest input first, or NULL for zero */
+    void *state_out;                              /* the window carried out, or NULL */
+} ssb_short_conv_t;
+typedef struct ssb_short_conv_grads {
+    ssb_view_t gout, gx;
+    const void *gstate_out;
+    void *gweight, *gbias, *gstate;               /* gbias, gstate optional */
+} ssb_short_conv_grads_t;
+int ssb_short_conv_fwd(const ssb_short_conv_t *p, void *stream);
+size_t ssb_short_conv_bwd_workspace_bytes(const ssb_short_conv_t *p);
+int ssb_short_conv_bwd(const ssb_short_conv_t *p, const ssb_short_conv_grads_t *g, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+typedef struct ssb_short_conv_step {
+    int dtype, silu, weight_f32;
+    int64_t entries, channels, width, pool;
+    const int32_t *slots;
+    ssb_view_t x, out;
+    const void *weight, *bias;
+    void *state;                                  /* [pool, C, W-1], updated in place */
+} ssb_short_conv_step_t;
+int ssb_short_conv_step(const ssb_short_conv_step_t *p, void *stream);
+
 /* Self-test of the bounded-wait machinery: launches one warp that looks back at a record which
  * is never published.  The kernel returns by itself after the poll's time limit (about one
  * second); afterwards ssb_device_status() reports SSB_ERR_DEVICE_WAIT once and the context

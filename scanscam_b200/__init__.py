@@ -8,14 +8,17 @@ live on a CUDA device and the native libraries must be built (``python -m scansc
 """
 import importlib
 
-__all__ = ["scan", "Scan", "is_transpose_contig", "scan_sigmoid_gate", "scan_recompute", "ScanRecompute"]
+__all__ = ["scan", "Scan", "is_transpose_contig", "scan_sigmoid_gate", "scan_recompute", "ScanRecompute",
+           "scan_selective", "scan_selective_step", "short_conv", "short_conv_step"]
 __version__ = "0.2.0"
 
 # The operator modules load the native extension when they are imported.  They are resolved on
 # first use, so that the helper modules that need no device (``workloads``, ``build``, ``_native``)
 # can be imported without pulling the CUDA libraries into the process.
 _LAZY = {"scan": "op", "Scan": "op", "is_transpose_contig": "op", "scan_sigmoid_gate": "fused",
-         "scan_recompute": "recompute", "ScanRecompute": "recompute"}
+         "scan_recompute": "recompute", "ScanRecompute": "recompute",
+         "scan_selective": "state_space", "scan_selective_step": "state_space", "short_conv": "state_space",
+         "short_conv_step": "state_space"}
 
 
 def __getattr__(name):

@@ -83,6 +83,15 @@ SIGNATURES = {
     "ssb_peer_buffer_destroy": (_int, [_p]),
     "ssb_shard_map_publish_f32": (_int, [_p, _p, _i64, _i64, ctypes.c_float, _int, _p, ctypes.c_uint, _p, _p]),
     "ssb_shard_carry_peer_f32": (_int, [_p, ctypes.c_uint, _int, _p, _p]),
+    "ssb_selective_checkpoint_bytes": (_sz, [_p]),
+    "ssb_selective_fwd": (_int, [_p, _p]),
+    "ssb_selective_bwd_workspace_bytes": (_sz, [_p]),
+    "ssb_selective_bwd": (_int, [_p, _p, _p, _sz, _p]),
+    "ssb_selective_step": (_int, [_p, _p]),
+    "ssb_short_conv_fwd": (_int, [_p, _p]),
+    "ssb_short_conv_bwd_workspace_bytes": (_sz, [_p]),
+    "ssb_short_conv_bwd": (_int, [_p, _p, _p, _sz, _p]),
+    "ssb_short_conv_step": (_int, [_p, _p]),
     "ssb_selftest_wait_timeout": (_int, [_p, _sz, _p]),
     "ssb_checked_build": (_int, []),
     "ssb_selftest_index_check": (_int, [_p]),
@@ -93,6 +102,65 @@ class PeerExchangeStruct(ctypes.Structure):
     """``ssb_peer_exchange_t``."""
 
     _fields_ = [("world", ctypes.c_int), ("rank", ctypes.c_int), ("rows", ctypes.c_int64), ("buffers", ctypes.c_void_p * 8)]
+
+
+F32, BF16, F16 = range(3)  # ssb_dtype_t
+
+
+def _fields(*spec):
+    """``("name other", type)`` groups -> the ``_fields_`` of a structure, in order."""
+    return [(name, kind) for names, kind in spec for name in names.split()]
+
+
+class View(ctypes.Structure):
+    """``ssb_view_t``."""
+
+    _fields_ = [("data", _p), ("stride", _i64 * 4)]
+
+
+class Selective(ctypes.Structure):
+    """``ssb_selective_t``."""
+
+    _fields_ = _fields(("dtype softplus", _int), ("batch channels steps states groups sequences", _i64), ("offsets lengths", _p),
+                       ("x dt z B C out", View), ("A D dt_bias state state_out checkpoints", _p))
+
+
+class SelectiveGrads(ctypes.Structure):
+    """``ssb_selective_grads_t``."""
+
+    _fields_ = _fields(("gout", View), ("gstate_out", _p), ("gx gdt gz gB gC", View), ("gA gD gdt_bias gstate", _p))
+
+
+class SelectiveStep(ctypes.Structure):
+    """``ssb_selective_step_t``."""
+
+    _fields_ = _fields(("dtype softplus", _int), ("entries channels states groups pool", _i64), ("slots", _p),
+                       ("x dt z B C out", View), ("A D dt_bias state", _p))
+
+
+class ShortConv(ctypes.Structure):
+    """``ssb_short_conv_t``."""
+
+    _fields_ = _fields(("dtype silu weight_f32", _int), ("batch channels steps width sequences", _i64), ("offsets lengths", _p),
+                       ("x out", View), ("weight bias state state_out", _p))
+
+
+class ShortConvGrads(ctypes.Structure):
+    """``ssb_short_conv_grads_t``."""
+
+    _fields_ = _fields(("gout gx", View), ("gstate_out gweight gbias gstate", _p))
+
+
+class ShortConvStep(ctypes.Structure):
+    """``ssb_short_conv_step_t``."""
+
+    _fields_ = _fields(("dtype silu weight_f32", _int), ("entries channels width pool", _i64), ("slots", _p), ("x out", View),
+                       ("weight bias state", _p))
+
+
+def view(t) -> View:
+    """A torch tensor's address and strides (an absent one for None)."""
+    return View() if t is None else View(t.data_ptr(), (_i64 * 4)(*t.stride()))
 
 
 _lib = None

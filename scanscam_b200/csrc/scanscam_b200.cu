@@ -15,6 +15,7 @@
 #include <limits>
 #include <type_traits>
 
+#include "host_common.h"
 #include "scan_cl.cuh"
 #include "scan_cl_lookback.cuh"
 #include "scan_cl_narrow.cuh"
@@ -30,8 +31,10 @@
 #include "scan_warp.cuh"
 
 namespace {
-
 thread_local char t_last_error[512] = "";
+}
+
+namespace ssb_host {
 
 int fail(int status, const char *fmt, ...) {
     va_list ap;
@@ -49,17 +52,6 @@ int check_launch(const char *what) {
     return SSB_OK;
 }
 
-bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
-// Validates a [rows, T] problem; *n receives rows*T.
-int check_shape(int64_t rows, int64_t T, int64_t *n) {
-    if (rows < 0 || T < 0) return fail(SSB_ERR_BAD_ARG, "negative size: rows=%lld T=%lld", (long long)rows, (long long)T);
-    if (T > 0 && rows > std::numeric_limits<int64_t>::max() / 8 / T)
-        return fail(SSB_ERR_BAD_ARG, "rows*T overflows: rows=%lld T=%lld", (long long)rows, (long long)T);
-    *n = rows * T;
-    return SSB_OK;
-}
-
 int sm_count() {
     static std::atomic<int> cached[64];
     int dev = 0;
@@ -70,6 +62,25 @@ int sm_count() {
         cached[dev].store(v, std::memory_order_relaxed);
     }
     return v;
+}
+
+}  // namespace ssb_host
+
+namespace {
+
+using ssb_host::check_launch;
+using ssb_host::fail;
+using ssb_host::sm_count;
+
+bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+// Validates a [rows, T] problem; *n receives rows*T.
+int check_shape(int64_t rows, int64_t T, int64_t *n) {
+    if (rows < 0 || T < 0) return fail(SSB_ERR_BAD_ARG, "negative size: rows=%lld T=%lld", (long long)rows, (long long)T);
+    if (T > 0 && rows > std::numeric_limits<int64_t>::max() / 8 / T)
+        return fail(SSB_ERR_BAD_ARG, "rows*T overflows: rows=%lld T=%lld", (long long)rows, (long long)T);
+    *n = rows * T;
+    return SSB_OK;
 }
 
 // ------------------------------------------------------------------------------------
@@ -2276,10 +2287,18 @@ int ssb_device_status(int *detail) {
     int word[2] = {0, 0};
     e = cudaMemcpyFromSymbol(word, ssb::g_status_word, sizeof(word));
     if (e != cudaSuccess) return fail(SSB_ERR_LAUNCH, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
-    if (detail) *detail = word[1];
+    int other[2] = {0, 0};
+    e = (cudaError_t)ssb_host::take_state_space_status(other);
+    if (e != cudaSuccess) return fail(SSB_ERR_LAUNCH, "cudaMemcpyFromSymbol: %s", cudaGetErrorString(e));
     if (word[0] != 0) {
         const int zero[2] = {0, 0};
         (void)cudaMemcpyToSymbol(ssb::g_status_word, zero, sizeof(zero));
+    } else {
+        word[0] = other[0];
+        word[1] = other[1];
+    }
+    if (detail) *detail = word[1];
+    if (word[0] != 0) {
         return word[0] == SSB_ERR_DEVICE_CHECK
                    ? fail(word[0], "a kernel computed an index outside its tensor and skipped the access (site %d)", word[1])
                    : fail(word[0], "a device-side wait ran out (kernel code %d)", word[1]);

@@ -1,0 +1,646 @@
+// Selective scan over whole sequences: per channel c and state n
+//     h_t = exp(dt_t A[c,n]) h_{t-1} + dt_t x_t B_t[n],     y_t = sum_n C_t[n] h_t + D x_t,     out = y silu(z),
+// and its backward, which runs the adjoint r_t = exp(dt_t A) (gy_t C_t + r_{t+1}) from the right.
+//
+// What bounds it: one exponential per (step, channel, state).  At 16 a clock and SM that is four
+// times what the tensors take to move in 16-bit storage, so the kernels are laid out around the
+// arithmetic: the states are never written to memory, and the recurrence is cut along time inside
+// the warp so that an exponential is computed once and used twice (fold and replay).
+//
+// A thread holds 8 consecutive steps of 2 adjacent channels (pairs in 64-bit registers) and goes
+// through the states one by one.  For a state it folds its 8 steps to an affine map, the TL lanes
+// that hold the same channels compose their maps with log2(TL) shuffle steps, and each thread then
+// replays its steps from the state that enters them, adding C_t h_t to its 16 sums: the sum over
+// states needs no communication.  A warp covers TL * 8 steps of 2 * 32 / TL channels; a CTA of W
+// warps W times the channels of the same steps, whose B and C it stages in shared memory as fp32.
+// TL is the split of the 32 lanes between time and channels: larger where there are few channels.
+#pragma once
+
+#include "ssm_common.cuh"
+
+namespace ssb {
+
+struct ProjView {  // B or C: [N, G, S, T]
+    void *data;
+    int64_t sn, sg, ss, st, extent;
+};
+
+struct SelectiveArgs {
+    int64_t channels, per_group, groups, states;
+    int blocks_per_group, softplus, slab, tile_log2;  // slab: states staged at a time; tile_log2: steps between checkpoints
+    Sequences seq;
+    View3 x, dt, z, out;
+    ProjView B, C;
+    const float *A, *D, *dt_bias, *state;
+    float *state_out, *checkpoints;
+    int64_t checkpoint_slots;
+};
+
+struct SelectiveGradArgs {
+    View3 gout, gx, gdt, gz;
+    const float *gstate_out;
+    float *gstate;
+    float *part_B, *part_C;  // [blocks per group][N, T, G, S]
+    float *part_A, *part_D, *part_bias;  // [gridDim.y][C, S], [gridDim.y][C] twice
+    int64_t rows;
+};
+
+constexpr int kSlab = 32;  // most states staged at a time
+
+__host__ __device__ constexpr int scan_pad(int tile) { return tile + 4; }  // floats per staged state: keeps 16-byte alignment
+
+// First checkpoint slot of a sequence: ceil(length / tile) slots from here never reach the next one's.
+__device__ __forceinline__ int64_t checkpoint_base(const SelectiveArgs &p, int64_t s, int64_t start) {
+    const int64_t per_row = (p.seq.steps + (1ll << p.tile_log2) - 1) >> p.tile_log2;
+    return p.seq.offsets != nullptr ? (start >> p.tile_log2) + s : s * per_row;
+}
+
+// Steps [t, t + tile) of states [n0, n0 + count) of B or C into shared memory, [state][step]; zero behind `steps`.
+template <typename io_t, int TILE>
+__device__ __forceinline__ void stage_projection(const ProjView &v, int64_t row, int64_t g, int n0, int count, int64_t t,
+                                                 int64_t steps, float *smem) {
+    const io_t *base = static_cast<const io_t *>(v.data);
+    const int64_t at = row * v.sn + g * v.sg + n0 * v.ss + t * v.st;
+    const int total = count * TILE;
+    for (int i = threadIdx.x; i < total; i += blockDim.x) {
+        int n, k;  // the index that is adjacent in memory runs over the lanes
+        if (v.ss == 1) {
+            k = i / count;
+            n = i - k * count;
+        } else {
+            n = i / TILE;
+            k = i % TILE;
+        }
+        smem[n * scan_pad(TILE) + k] = k < steps ? load_one<io_t>(base, at + n * v.ss + k * v.st, v.extent, 210) : 0.0f;
+    }
+}
+
+// A[c, n] * log2(e) of the CTA's channels, [state][channel]; zero behind the last channel.  An
+// infinite entry becomes the largest finite one: with a step of zero it then decays by 2^0 = 1, as
+// padding has to.
+template <int CB>
+__device__ __forceinline__ void stage_decays(const SelectiveArgs &p, int64_t c0, int64_t c_end, int n0, int count, float *smem) {
+    for (int i = threadIdx.x; i < count * CB; i += blockDim.x) {
+        const int c = i / count, n = i - c * count;
+        float v = 0.0f;
+        if (c0 + c < c_end) {
+            const int64_t at = (c0 + c) * p.states + n0 + n;
+            if (SSB_INDEX_OK(at, p.channels * p.states, 211)) v = p.A[at] * kLog2e;
+            if (isinf(v)) v = copysignf(3.402823466e38f, v);
+        }
+        smem[n * CB + c] = v;
+    }
+}
+
+// Zeros into steps [from, to) of a row of the CTA's channels.
+template <typename io_t>
+__device__ __forceinline__ void zero_steps(const View3 &v, int64_t row, int64_t c0, int64_t c_end, int64_t from, int64_t to, int site) {
+    io_t *base = static_cast<io_t *>(v.data);
+    const int64_t nc = c_end - c0, nt = to - from;
+    if (nc <= 0 || nt <= 0) return;
+    for (int64_t i = threadIdx.x; i < nc * nt; i += blockDim.x) {
+        int64_t c, t;
+        if (v.sc == 1) {
+            t = i / nc;
+            c = i - t * nc;
+        } else {
+            c = i / nt;
+            t = i - c * nt;
+        }
+        store_one<io_t>(base, row * v.sn + (c0 + c) * v.sc + (from + t) * v.st, v.extent, site, 0.0f);
+    }
+}
+
+// The steps of an output that belong to no sequence are zero: behind a row's length, before the
+// first packed sequence and behind the last.
+template <typename io_t>
+__device__ __forceinline__ void zero_uncovered(const Sequences &q, int64_t s, const Span &sp, const View3 &v, int64_t c0,
+                                               int64_t c_end, int site) {
+    if (q.offsets == nullptr) {
+        zero_steps<io_t>(v, sp.row, c0, c_end, sp.length, q.steps, site);
+    } else {
+        if (s == 0) zero_steps<io_t>(v, 0, c0, c_end, 0, sp.start, site);
+        if (s == q.count - 1) zero_steps<io_t>(v, 0, c0, c_end, sp.start + sp.length, q.steps, site);
+    }
+}
+
+// Per-channel [C, S] values of a warp's own channels between global memory and [state][channel] in shared memory.
+template <int CB, int CW>
+__device__ __forceinline__ void load_states(const float *src, int64_t seq, const SelectiveArgs &p, int64_t c0, int64_t c_end,
+                                            int warp, int lane, int site, float *smem) {
+    for (int i = lane; i < CW * (int)p.states; i += 32) {
+        const int c = i / (int)p.states, n = i - c * (int)p.states, cl = warp * CW + c;
+        float v = 0.0f;
+        if (src != nullptr && c0 + cl < c_end) {
+            const int64_t at = (seq * p.channels + c0 + cl) * p.states + n;
+            if (SSB_INDEX_OK(at, p.seq.count * p.channels * p.states, site)) v = src[at];
+        }
+        smem[n * CB + cl] = v;
+    }
+    __syncwarp();
+}
+template <int CB, int CW>
+__device__ __forceinline__ void store_states(float *dst, int64_t seq, const SelectiveArgs &p, int64_t c0, int64_t c_end,
+                                             int warp, int lane, int site, const float *smem) {
+    __syncwarp();
+    for (int i = lane; i < CW * (int)p.states; i += 32) {
+        const int c = i / (int)p.states, n = i - c * (int)p.states, cl = warp * CW + c;
+        if (c0 + cl < c_end) {
+            const int64_t at = (seq * p.channels + c0 + cl) * p.states + n;
+            if (SSB_INDEX_OK(at, p.seq.count * p.channels * p.states, site)) dst[at] = smem[n * CB + cl];
+        }
+    }
+    __syncwarp();
+}
+
+// The step sizes of a run: softplus(raw + bias) or raw + bias; zero (decay 1, no input) behind the last step.
+__device__ __forceinline__ void make_steps(pair_t (&dt)[kRun], float2 bias, int softplus_on, int steps) {
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+        float2 f = halves(dt[k]);
+        f.x += bias.x;
+        f.y += bias.y;
+        if (softplus_on) {
+            f.x = softplus(f.x);
+            f.y = softplus(f.y);
+        }
+        dt[k] = k < steps ? make_pair(f.x, f.y) : 0;
+    }
+}
+
+// Composes the maps (P, S) of a channel's TL lanes from the left: inclusive prefix.
+template <int TL>
+__device__ __forceinline__ void compose_left(pair_t &P, pair_t &S, int tl) {
+    constexpr int DL = 32 / TL;
+#pragma unroll
+    for (int d = 1; d < TL; d <<= 1) {
+        const pair_t P0 = shfl_up2(P, d * DL), S0 = shfl_up2(S, d * DL);
+        if (tl >= d) {
+            S = fma2(P, S0, S);
+            P = mul2(P, P0);
+        }
+    }
+}
+template <int TL>
+__device__ __forceinline__ void compose_right(pair_t &P, pair_t &S, int tl) {
+    constexpr int DL = 32 / TL;
+#pragma unroll
+    for (int d = 1; d < TL; d <<= 1) {
+        const pair_t P0 = shfl_down2(P, d * DL), S0 = shfl_down2(S, d * DL);
+        if (tl + d < TL) {
+            S = fma2(P, S0, S);
+            P = mul2(P, P0);
+        }
+    }
+}
+
+__device__ __forceinline__ void load8(const float *smem, float (&v)[kRun]) {
+    const float4 a = *reinterpret_cast<const float4 *>(smem), b = *reinterpret_cast<const float4 *>(smem + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+template <int TL, int W>
+struct ScanShape {
+    static constexpr int DL = 32 / TL;       // lanes across channels
+    static constexpr int CW = 2 * DL;        // channels of a warp
+    static constexpr int CB = W * CW;        // channels of a CTA
+    static constexpr int TILE = TL * kRun;   // steps of a tile
+    static constexpr int PAD = scan_pad(TILE);
+};
+
+template <int TL, int W>
+__host__ __device__ constexpr size_t selective_fwd_smem(int64_t states, int slab) {
+    using H = ScanShape<TL, W>;
+    return sizeof(float) * ((size_t)states * H::CB + (size_t)slab * (H::CB + 2 * H::PAD));
+}
+
+template <typename io_t, int TL, int W>
+__global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
+    using H = ScanShape<TL, W>;
+    extern __shared__ __align__(16) float smem[];
+    float *carry = smem;                                   // [states][CB]: the state entering the tile
+    float *decay = carry + p.states * H::CB;               // [slab][CB]
+    float *Bs = decay + p.slab * H::CB, *Cs = Bs + p.slab * H::PAD;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tl = lane / H::DL, cl = warp * H::CW + 2 * (lane % H::DL);
+    const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
+    const int64_t c0 = g * p.per_group + j * H::CB;
+    const int64_t c_end = c0 + H::CB < (g + 1) * p.per_group ? c0 + H::CB : (g + 1) * p.per_group;
+    const int64_t c = c0 + cl;
+    const int nc = c_end - c >= 2 ? 2 : (c_end > c ? 1 : 0);  // channels of this thread that exist
+    const int S = (int)p.states;
+    float2 D = make_float2(0.0f, 0.0f), bias = D;
+    if (p.D != nullptr) {
+        if (nc > 0) D.x = load_one(p.D, c, p.channels, 212);
+        if (nc > 1) D.y = load_one(p.D, c + 1, p.channels, 212);
+    }
+    if (p.dt_bias != nullptr) {
+        if (nc > 0) bias.x = load_one(p.dt_bias, c, p.channels, 213);
+        if (nc > 1) bias.y = load_one(p.dt_bias, c + 1, p.channels, 213);
+    }
+    if (S <= p.slab) {  // staged once for all tiles
+        stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
+    }
+
+    for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
+        const Span sp = span_of(p.seq, s);
+        load_states<H::CB, H::CW>(p.state, s, p, c0, c_end, warp, lane, 214, carry);
+        const int64_t slot0 = p.checkpoints != nullptr ? checkpoint_base(p, s, sp.start) : 0;
+        for (int64_t t0 = 0; t0 < sp.length; t0 += H::TILE) {
+            const int64_t left = sp.length - t0 - tl * kRun;
+            const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
+            const int64_t t = sp.start + t0 + tl * kRun;
+            pair_t dt[kRun], u[kRun], y[kRun];
+            load_run<io_t>(p.x, sp.row, c, t, steps, nc, 215, u);
+            load_run<io_t>(p.dt, sp.row, c, t, steps, nc, 216, dt);
+            make_steps(dt, bias, p.softplus, steps);
+            const pair_t Dp = make_pair(D.x, D.y);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                y[k] = mul2(Dp, u[k]);
+                u[k] = mul2(dt[k], u[k]);  // from here on dt * x
+            }
+            if (p.checkpoints != nullptr && (t0 & ((1ll << p.tile_log2) - 1)) == 0) {
+                const int64_t slot = slot0 + (t0 >> p.tile_log2);
+                for (int n = tl; n < S; n += TL) {
+                    const int64_t at = (slot * S + n) * p.channels + c;
+                    const float *from = carry + n * H::CB + cl;
+                    if (nc > 0) store_one(p.checkpoints, at, p.checkpoint_slots * S * p.channels, 217, from[0]);
+                    if (nc > 1) store_one(p.checkpoints, at + 1, p.checkpoint_slots * S * p.channels, 217, from[1]);
+                }
+                __syncwarp();
+            }
+            for (int n0 = 0; n0 < S; n0 += p.slab) {
+                const int count = S - n0 < p.slab ? S - n0 : p.slab;
+                __syncthreads();
+                if (S > p.slab) stage_decays<H::CB>(p, c0, c_end, n0, count, decay);
+                stage_projection<io_t, H::TILE>(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
+                stage_projection<io_t, H::TILE>(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
+                __syncthreads();
+                for (int n = 0; n < count; ++n) {
+                    const pair_t A = *reinterpret_cast<const pair_t *>(decay + n * H::CB + cl);
+                    pair_t *held = reinterpret_cast<pair_t *>(carry + (n0 + n) * H::CB + cl);
+                    const pair_t h_in = *held;
+                    pair_t a[kRun], b[kRun];
+                    float v[kRun];
+                    load8(Bs + n * H::PAD + tl * kRun, v);
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) {
+                        a[k] = exp2_pair(mul2(dt[k], A));
+                        b[k] = mul2(u[k], both(v[k]));
+                    }
+                    pair_t P = a[0], F = b[0];
+#pragma unroll
+                    for (int k = 1; k < kRun; ++k) {
+                        F = fma2(a[k], F, b[k]);
+                        P = mul2(P, a[k]);
+                    }
+                    compose_left<TL>(P, F, tl);
+                    const pair_t h_end = fma2(P, h_in, F);  // the state behind this lane's steps
+                    pair_t h = shfl_up2(h_end, H::DL);
+                    if (tl == 0) h = h_in;
+                    __syncwarp();
+                    if (tl == TL - 1) *held = h_end;
+                    load8(Cs + n * H::PAD + tl * kRun, v);
+#pragma unroll
+                    for (int k = 0; k < kRun; ++k) {
+                        h = fma2(a[k], h, b[k]);
+                        y[k] = fma2(h, both(v[k]), y[k]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (p.z.data != nullptr) {
+                load_run<io_t>(p.z, sp.row, c, t, steps, nc, 218, u);
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) {
+                    const float2 z = halves(u[k]), f = halves(y[k]);
+                    y[k] = make_pair(f.x * (z.x * logistic(z.x)), f.y * (z.y * logistic(z.y)));
+                }
+            }
+            store_run<io_t>(p.out, sp.row, c, t, steps, nc, 219, y);
+        }
+        if (p.state_out != nullptr) store_states<H::CB, H::CW>(p.state_out, s, p, c0, c_end, warp, lane, 220, carry);
+        zero_uncovered<io_t>(p.seq, s, sp, p.out, c0, c_end, 219);
+        __syncthreads();  // the staged tile of this sequence is no longer read
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------
+// Tiles run from the last to the first.  Each starts from its checkpoint (the state the forward
+// wrote at the tile's first step), rebuilds the states as the forward does, and carries the adjoint
+// r to the tile on its left.  Per (step, channel, state) there is one exponential and 17 fp32
+// operations, so the fp32 pipe bounds it, not the special function unit.
+//
+// The gradients of B and C sum over channels: over the pair in the thread, over the DL lanes by an
+// exchange that halves the number of values at each step (16 values: 8 + 4 shuffles for DL = 4),
+// over the warps of the CTA in shared memory, over CTAs by selective_reduce_kernel in a fixed order.  The warps of
+// a CTA work on different states at a time (warp w on state (i + w) mod count), with a barrier per
+// state, so that none adds to a row of sums that another is adding to, and the order of the additions is always the same.
+template <int TL, int W>
+__host__ __device__ constexpr size_t selective_bwd_smem(int64_t states, int slab) {
+    using H = ScanShape<TL, W>;
+    return sizeof(float) * ((size_t)states * H::CB * 2 + (size_t)slab * (2 * H::CB + 4 * H::PAD));
+}
+
+template <typename io_t, int TL, int W>
+__global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_constant__ SelectiveArgs p,
+                                                              const __grid_constant__ SelectiveGradArgs q) {
+    using H = ScanShape<TL, W>;
+    extern __shared__ __align__(16) float smem[];
+    float *adjoint = smem;                              // [states][CB]: r entering the tile from the right
+    float *gA = adjoint + p.states * H::CB;             // [states][CB]: sums over this CTA's steps
+    float *decay = gA + p.states * H::CB;               // [slab][CB]
+    float *first = decay + p.slab * H::CB;              // [slab][CB]: the state entering the tile
+    float *Bs = first + p.slab * H::CB, *Cs = Bs + p.slab * H::PAD;
+    float *sumB = Cs + p.slab * H::PAD, *sumC = sumB + p.slab * H::PAD;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int tl = lane / H::DL, dl = lane % H::DL, cl = warp * H::CW + 2 * dl;
+    const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
+    const int64_t c0 = g * p.per_group + j * H::CB;
+    const int64_t c_end = c0 + H::CB < (g + 1) * p.per_group ? c0 + H::CB : (g + 1) * p.per_group;
+    const int64_t c = c0 + cl;
+    const int nc = c_end - c >= 2 ? 2 : (c_end > c ? 1 : 0);
+    const int S = (int)p.states;
+    float2 D = make_float2(0.0f, 0.0f), bias = D;
+    if (p.D != nullptr) {
+        if (nc > 0) D.x = load_one(p.D, c, p.channels, 230);
+        if (nc > 1) D.y = load_one(p.D, c + 1, p.channels, 230);
+    }
+    if (p.dt_bias != nullptr) {
+        if (nc > 0) bias.x = load_one(p.dt_bias, c, p.channels, 231);
+        if (nc > 1) bias.y = load_one(p.dt_bias, c + 1, p.channels, 231);
+    }
+    const pair_t Dp = make_pair(D.x, D.y);
+    for (int i = threadIdx.x; i < S * H::CB; i += blockDim.x) gA[i] = 0.0f;
+    if (S <= p.slab) stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
+    pair_t gD = 0, gbias = 0;
+
+    for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
+        const Span sp = span_of(p.seq, s);
+        load_states<H::CB, H::CW>(q.gstate_out, s, p, c0, c_end, warp, lane, 232, adjoint);
+        const int64_t slot0 = checkpoint_base(p, s, sp.start);
+        const int64_t tiles = (sp.length + H::TILE - 1) / H::TILE;
+        for (int64_t i_tile = tiles - 1; i_tile >= 0; --i_tile) {
+            const int64_t t0 = i_tile * H::TILE;
+            const int64_t left = sp.length - t0 - tl * kRun;
+            const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
+            const int64_t t = sp.start + t0 + tl * kRun;
+            pair_t dt[kRun], u[kRun], gy[kRun], y[kRun];
+            pair_t through[kRun], bydecay[kRun];  // sum_n dh B  and  sum_n dh (a h_{t-1}) A log2(e)
+            load_run<io_t>(q.gout, sp.row, c, t, steps, nc, 233, gy);
+            if (p.z.data != nullptr) {
+                load_run<io_t>(p.z, sp.row, c, t, steps, nc, 234, y);
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) {
+                    const float2 z = halves(y[k]), f = halves(gy[k]);
+                    gy[k] = make_pair(f.x * (z.x * logistic(z.x)), f.y * (z.y * logistic(z.y)));
+                }
+            }
+            load_run<io_t>(p.x, sp.row, c, t, steps, nc, 235, u);
+            load_run<io_t>(p.dt, sp.row, c, t, steps, nc, 236, dt);
+            make_steps(dt, bias, p.softplus, steps);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                y[k] = mul2(Dp, u[k]);
+                gD = fma2(gy[k], u[k], gD);
+                u[k] = mul2(dt[k], u[k]);
+                through[k] = 0;
+                bydecay[k] = 0;
+            }
+            for (int n0 = 0; n0 < S; n0 += p.slab) {
+                const int count = S - n0 < p.slab ? S - n0 : p.slab;
+                __syncthreads();
+                if (S > p.slab) stage_decays<H::CB>(p, c0, c_end, n0, count, decay);
+                stage_projection<io_t, H::TILE>(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
+                stage_projection<io_t, H::TILE>(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
+                for (int i = threadIdx.x; i < count * H::CB; i += blockDim.x) {
+                    const int n = i / H::CB, cc = i % H::CB;
+                    const int64_t at = ((slot0 + i_tile) * S + n0 + n) * p.channels + c0 + cc;
+                    first[i] = c0 + cc < c_end ? load_one(p.checkpoints, at, p.checkpoint_slots * S * p.channels, 237) : 0.0f;
+                }
+                for (int i = threadIdx.x; i < count * H::PAD; i += blockDim.x) {
+                    sumB[i] = 0.0f;
+                    sumC[i] = 0.0f;
+                }
+                __syncthreads();
+                const int turns = count > W ? count : W;
+                for (int turn = 0; turn < turns; ++turn) {
+                    int n = turn + warp;
+                    if (n >= turns) n -= turns;
+                    if (n < count) {
+                        const pair_t A = *reinterpret_cast<const pair_t *>(decay + n * H::CB + cl);
+                        pair_t *held = reinterpret_cast<pair_t *>(adjoint + (n0 + n) * H::CB + cl);
+                        const pair_t r_in = *held;
+                        const pair_t h_in = *reinterpret_cast<const pair_t *>(first + n * H::CB + cl);
+                        pair_t a[kRun], m[kRun];
+                        float bv[kRun], cv[kRun], v[2 * kRun];
+                        load8(Bs + n * H::PAD + tl * kRun, bv);
+                        load8(Cs + n * H::PAD + tl * kRun, cv);
+#pragma unroll
+                        for (int k = 0; k < kRun; ++k) a[k] = exp2_pair(mul2(dt[k], A));
+                        pair_t P = a[0], F = mul2(u[0], both(bv[0]));
+#pragma unroll
+                        for (int k = 1; k < kRun; ++k) {
+                            F = fma2(u[k], both(bv[k]), mul2(a[k], F));
+                            P = mul2(P, a[k]);
+                        }
+                        const pair_t P0 = P;
+                        compose_left<TL>(P, F, tl);
+                        pair_t h = shfl_up2(fma2(P, h_in, F), H::DL);
+                        if (tl == 0) h = h_in;
+#pragma unroll
+                        for (int k = 0; k < kRun; ++k) {
+                            m[k] = mul2(a[k], h);                    // a_t h_{t-1}
+                            h = fma2(u[k], both(bv[k]), m[k]);
+                            y[k] = fma2(h, both(cv[k]), y[k]);
+                            const float2 f = halves(mul2(gy[k], h));
+                            v[kRun + k] = f.x + f.y;                 // this pair's part of the gradient of C
+                        }
+                        pair_t Q = 0;
+#pragma unroll
+                        for (int k = kRun - 1; k >= 0; --k) Q = mul2(a[k], fma2(gy[k], both(cv[k]), Q));
+                        P = P0;
+                        compose_right<TL>(P, Q, tl);
+                        const pair_t r_out = fma2(P, r_in, Q);       // r of this lane's first step
+                        pair_t r = shfl_down2(r_out, H::DL);
+                        if (tl == TL - 1) r = r_in;
+                        __syncwarp();
+                        if (tl == 0) *held = r_out;
+                        pair_t dA = 0;
+#pragma unroll
+                        for (int k = kRun - 1; k >= 0; --k) {
+                            const pair_t dh = fma2(gy[k], both(cv[k]), r);
+                            r = mul2(a[k], dh);
+                            const float2 f = halves(mul2(dh, u[k]));
+                            v[k] = f.x + f.y;                        // this pair's part of the gradient of B
+                            through[k] = fma2(dh, both(bv[k]), through[k]);
+                            const pair_t w = mul2(dh, m[k]);
+                            bydecay[k] = fma2(w, A, bydecay[k]);
+                            dA = fma2(w, dt[k], dA);
+                        }
+#pragma unroll
+                        for (int d = H::DL; d < 32; d <<= 1) {       // over the lanes of the channel
+                            const float2 f = halves(dA);
+                            dA = add2(dA, make_pair(__shfl_xor_sync(kFullMask, f.x, d), __shfl_xor_sync(kFullMask, f.y, d)));
+                        }
+                        if (tl == 0) {
+                            pair_t *to = reinterpret_cast<pair_t *>(gA + (n0 + n) * H::CB + cl);
+                            *to = add2(*to, dA);
+                        }
+                        // over the DL lanes: each ends with 16 / DL of the 16 sums
+                        int at = 0, held_values = 2 * kRun;
+#pragma unroll
+                        for (int bit = H::DL / 2; bit >= 1; bit >>= 1) {
+                            held_values >>= 1;
+                            const bool upper = (dl & bit) != 0;
+                            if (upper) at += held_values;
+#pragma unroll
+                            for (int i = 0; i < kRun; ++i) {
+                                if (i < held_values) {
+                                    const float give = upper ? v[i] : v[i + held_values];
+                                    const float keep = upper ? v[i + held_values] : v[i];
+                                    v[i] = keep + __shfl_xor_sync(kFullMask, give, bit);
+                                }
+                            }
+                        }
+                        constexpr int kHeld = 2 * kRun / H::DL;
+#pragma unroll
+                        for (int i = 0; i < kHeld; ++i) {
+                            const int w = at + i;
+                            float *to = (w < kRun ? sumB : sumC) + n * H::PAD + tl * kRun + (w & (kRun - 1));
+                            *to += v[i];
+                        }
+                    }
+                    __syncthreads();
+                }
+                // the CTA's sums: [block][row, step, group, state]
+                const int64_t extent = (int64_t)p.blocks_per_group * q.rows * p.seq.steps * p.groups * S;
+                const int valid = sp.length - t0 < H::TILE ? (int)(sp.length - t0) : H::TILE;
+                for (int i = threadIdx.x; i < count * valid; i += blockDim.x) {
+                    const int k = i / count, n = i - k * count;
+                    const int64_t at = (((j * q.rows + sp.row) * p.seq.steps + sp.start + t0 + k) * p.groups + g) * S + n0 + n;
+                    store_one(q.part_B, at, extent, 238, sumB[n * H::PAD + k]);
+                    store_one(q.part_C, at, extent, 239, sumC[n * H::PAD + k]);
+                }
+            }
+            // per step and channel: the gradients of x, dt, z
+            pair_t raw[kRun], xv[kRun], t2[kRun];
+            load_run<io_t>(p.x, sp.row, c, t, steps, nc, 235, xv);
+            load_run<io_t>(p.dt, sp.row, c, t, steps, nc, 236, raw);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                t2[k] = fma2(through[k], dt[k], mul2(Dp, gy[k]));
+                float2 f = halves(fma2(through[k], xv[k], mul2(bydecay[k], both(kLn2))));
+                if (p.softplus) {
+                    const float2 w = halves(raw[k]);
+                    f.x *= logistic_accurate(w.x + bias.x);
+                    f.y *= logistic_accurate(w.y + bias.y);
+                }
+                raw[k] = make_pair(f.x, f.y);
+                if (k < steps) gbias = add2(gbias, raw[k]);
+            }
+            store_run<io_t>(q.gx, sp.row, c, t, steps, nc, 240, t2);
+            store_run<io_t>(q.gdt, sp.row, c, t, steps, nc, 241, raw);
+            if (p.z.data != nullptr) {
+                load_run<io_t>(p.z, sp.row, c, t, steps, nc, 234, xv);
+                load_run<io_t>(q.gout, sp.row, c, t, steps, nc, 233, raw);
+#pragma unroll
+                for (int k = 0; k < kRun; ++k) {
+                    const float2 z = halves(xv[k]), f = halves(mul2(raw[k], y[k]));
+                    const float sx = logistic(z.x), sy = logistic(z.y);
+                    t2[k] = make_pair(f.x * sx * fmaf(z.x, 1.0f - sx, 1.0f), f.y * sy * fmaf(z.y, 1.0f - sy, 1.0f));
+                }
+                store_run<io_t>(q.gz, sp.row, c, t, steps, nc, 242, t2);
+            }
+        }
+        if (q.gstate != nullptr) store_states<H::CB, H::CW>(q.gstate, s, p, c0, c_end, warp, lane, 243, adjoint);
+        zero_uncovered<io_t>(p.seq, s, sp, q.gx, c0, c_end, 240);
+        zero_uncovered<io_t>(p.seq, s, sp, q.gdt, c0, c_end, 241);
+        if (p.z.data != nullptr) zero_uncovered<io_t>(p.seq, s, sp, q.gz, c0, c_end, 242);
+        __syncthreads();
+    }
+    // this CTA's sums over its steps
+    __syncthreads();
+    for (int i = threadIdx.x; i < S * H::CB; i += blockDim.x) {
+        const int cc = i / S, n = i - cc * S;
+        if (c0 + cc < c_end)
+            store_one(q.part_A, ((int64_t)blockIdx.y * p.channels + c0 + cc) * S + n, (int64_t)gridDim.y * p.channels * S, 244,
+                      gA[n * H::CB + cc]);
+    }
+#pragma unroll
+    for (int d = H::DL; d < 32; d <<= 1) {
+        const float2 f = halves(gD), b = halves(gbias);
+        gD = add2(gD, make_pair(__shfl_xor_sync(kFullMask, f.x, d), __shfl_xor_sync(kFullMask, f.y, d)));
+        gbias = add2(gbias, make_pair(__shfl_xor_sync(kFullMask, b.x, d), __shfl_xor_sync(kFullMask, b.y, d)));
+    }
+    if (tl == 0) {
+        const float2 f = halves(gD), b = halves(gbias);
+        const int64_t at = (int64_t)blockIdx.y * p.channels + c, extent = (int64_t)gridDim.y * p.channels;
+        if (nc > 0) {
+            store_one(q.part_D, at, extent, 245, f.x);
+            store_one(q.part_bias, at, extent, 246, b.x);
+        }
+        if (nc > 1) {
+            store_one(q.part_D, at + 1, extent, 245, f.y);
+            store_one(q.part_bias, at + 1, extent, 246, b.y);
+        }
+    }
+}
+
+// Sums the CTAs' parts, in the order of their numbers: B and C over the channel blocks of a group
+// (blocks [0, proj_blocks) of the grid), A, D and dt_bias over the CTAs that shared the sequences.
+// Steps that no sequence covers were not written and give zero.
+struct SelectiveReduceArgs {
+    Sequences seq;
+    int64_t rows, groups, states, channels;
+    int parts_proj, parts_seq, proj_blocks;
+    const float *part_B, *part_C, *part_A, *part_D, *part_bias;
+    ProjView gB, gC;
+    float *gA, *gD, *gbias;
+};
+
+__device__ __forceinline__ bool step_covered(const Sequences &q, int64_t row, int64_t t) {
+    if (q.offsets != nullptr) {  // sequences follow one another
+        const int64_t a = clamp_step(q.offsets[0], 0, q.steps), b = clamp_step(q.offsets[q.count], a, q.steps);
+        return t >= a && t < b;
+    }
+    return q.lengths == nullptr || t < clamp_step(q.lengths[row], 0, q.steps);
+}
+
+template <typename io_t>
+__global__ void __launch_bounds__(256) selective_reduce_kernel(const __grid_constant__ SelectiveReduceArgs p) {
+    const int64_t each = p.rows * p.seq.steps * p.groups * p.states;
+    if ((int)blockIdx.x < p.proj_blocks) {
+        for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < each; i += (int64_t)p.proj_blocks * blockDim.x) {
+            const int64_t n = i % p.states, g = i / p.states % p.groups, rt = i / (p.states * p.groups);
+            const int64_t t = rt % p.seq.steps, row = rt / p.seq.steps;
+            float b = 0.0f, c = 0.0f;
+            if (step_covered(p.seq, row, t)) {
+#pragma unroll 4
+                for (int j = 0; j < p.parts_proj; ++j) {
+                    b += load_one(p.part_B, j * each + i, p.parts_proj * each, 250);
+                    c += load_one(p.part_C, j * each + i, p.parts_proj * each, 251);
+                }
+            }
+            store_one(static_cast<io_t *>(p.gB.data), row * p.gB.sn + g * p.gB.sg + n * p.gB.ss + t * p.gB.st, p.gB.extent, 252, b);
+            store_one(static_cast<io_t *>(p.gC.data), row * p.gC.sn + g * p.gC.sg + n * p.gC.ss + t * p.gC.st, p.gC.extent, 253, c);
+        }
+    } else {
+        const int64_t cs = p.channels * p.states, total = cs + 2 * p.channels;
+        const int64_t stride = (int64_t)(gridDim.x - p.proj_blocks) * blockDim.x;
+        for (int64_t i = (int64_t)(blockIdx.x - p.proj_blocks) * blockDim.x + threadIdx.x; i < total; i += stride) {
+            const float *part = i < cs ? p.part_A : (i < cs + p.channels ? p.part_D : p.part_bias);
+            float *to = i < cs ? p.gA : (i < cs + p.channels ? p.gD : p.gbias);
+            const int64_t size = i < cs ? cs : p.channels, at = i < cs ? i : (i - cs) % p.channels;
+            if (to == nullptr) continue;
+            float v = 0.0f;
+#pragma unroll 4
+            for (int j = 0; j < p.parts_seq; ++j) v += load_one(part, j * size + at, p.parts_seq * size, 254);
+            store_one(to, at, size, 255, v);
+        }
+    }
+}
+
+}  // namespace ssb

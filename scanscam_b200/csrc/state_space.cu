@@ -1,0 +1,586 @@
+// C-ABI entry points of the state-space operators: argument checks, choice of the kernel's shape,
+// launches.  Kernels: ssm_scan.cuh, ssm_step.cuh, short_conv.cuh.
+#include "../../include/scanscam_b200.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <limits>
+
+#include "host_common.h"
+#include "short_conv.cuh"
+#include "ssm_scan.cuh"
+#include "ssm_step.cuh"
+
+using ssb_host::check_launch;
+using ssb_host::fail;
+using ssb_host::sm_count;
+
+namespace {
+
+constexpr int64_t kMaxStates = 256;
+constexpr size_t kSmemLimit = 227 * 1024;
+
+size_t size_of(int dtype) { return dtype == SSB_F32 ? 4 : 2; }
+bool aligned(const void *p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Calls f with a null pointer of the storage type.
+template <typename F>
+int with_type(int dtype, F &&f) {
+    if (dtype == SSB_F32) return f(static_cast<float *>(nullptr));
+    if (dtype == SSB_BF16) return f(static_cast<__nv_bfloat16 *>(nullptr));
+    return f(static_cast<__half *>(nullptr));
+}
+
+int check_sizes(int dtype, std::initializer_list<int64_t> sizes) {
+    if (dtype != SSB_F32 && dtype != SSB_BF16 && dtype != SSB_F16) return fail(SSB_ERR_BAD_ARG, "unknown element type %d", dtype);
+    int64_t all = 1;
+    for (int64_t s : sizes) {
+        if (s < 0) return fail(SSB_ERR_BAD_ARG, "negative size: %lld", (long long)s);
+        if (s > 0 && all > std::numeric_limits<int64_t>::max() / 64 / s) return fail(SSB_ERR_BAD_ARG, "sizes overflow");
+        if (s > 0) all *= s;
+    }
+    return SSB_OK;
+}
+
+int check_sequences(int64_t batch, int64_t sequences, const int32_t *offsets, const int32_t *lengths) {
+    if (offsets == nullptr) return SSB_OK;
+    if (lengths != nullptr) return fail(SSB_ERR_BAD_ARG, "offsets and lengths exclude each other");
+    if (batch != 1) return fail(SSB_ERR_BAD_ARG, "packed sequences need a batch of 1, got %lld", (long long)batch);
+    if (sequences < 1) return fail(SSB_ERR_BAD_ARG, "offsets must bound at least one sequence, got %lld", (long long)sequences);
+    return SSB_OK;
+}
+
+ssb::Sequences sequences_of(int64_t batch, int64_t steps, int64_t sequences, const int32_t *offsets, const int32_t *lengths) {
+    return {offsets, lengths, offsets != nullptr ? sequences : batch, steps};
+}
+
+int check_data(const void *p, int dtype, const char *name) {
+    if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "%s is NULL", name);
+    if (!aligned(p, size_of(dtype))) return fail(SSB_ERR_ALIGNMENT, "%s is not aligned to its element size", name);
+    return SSB_OK;
+}
+
+int64_t extent_of(const ssb_view_t &v, std::initializer_list<int64_t> sizes) {
+    int64_t last = 0;
+    int i = 0;
+    for (int64_t s : sizes) last += (s - 1) * v.stride[i++];
+    return last + 1;
+}
+
+// A [N, C, T] view and how runs of it may be fetched.  `from_zero`: every run starts at a multiple of
+// 8 steps; `even`: every pair of channels starts at an even one (not so in groups of an odd size).
+ssb::View3 view3(const ssb_view_t &v, int dtype, int64_t n, int64_t c, int64_t t, bool from_zero, bool even) {
+    const size_t e = size_of(dtype);
+    ssb::View3 r{v.data, v.stride[0], v.stride[1], v.stride[2], v.data != nullptr ? extent_of(v, {n, c, t}) : 0, ssb::kAnyStride};
+    if (even && v.stride[1] == 1 && v.stride[2] % 2 == 0 && v.stride[0] % 2 == 0 && aligned(v.data, 2 * e)) r.access = ssb::kPairs;
+    else if (v.stride[2] == 1 && from_zero && v.stride[1] % 8 == 0 && v.stride[0] % 8 == 0 && aligned(v.data, 16)) r.access = ssb::kRuns;
+    return r;
+}
+ssb::ProjView proj_view(const ssb_view_t &v, int64_t n, int64_t g, int64_t s, int64_t t) {
+    return {v.data, v.stride[0], v.stride[1], v.stride[2], v.stride[3], v.data != nullptr ? extent_of(v, {n, g, s, t}) : 0};
+}
+ssb::View2 view2(const ssb_view_t &v, int64_t a, int64_t b, int64_t c = 1) {
+    return {v.data, v.stride[0], v.stride[1], v.stride[2], v.data != nullptr ? extent_of(v, {a, b, c}) : 0};
+}
+
+template <typename K>
+int allow_smem(K kernel, size_t bytes) {
+    if (bytes <= 48 * 1024) return SSB_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == cudaSuccess ? SSB_OK : fail(SSB_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+}
+
+// ---- selective scan -----------------------------------------------------------------------------
+constexpr int kFwdWarps = 4, kBwdWarps = 8;
+
+// Calls f with the split of a warp between time and channels as a compile-time constant.
+template <typename F>
+auto with_split(int tl, F &&f) {
+    switch (tl) {
+        case 4: return f(std::integral_constant<int, 4>{});
+        case 8: return f(std::integral_constant<int, 8>{});
+        case 16: return f(std::integral_constant<int, 16>{});
+        default: return f(std::integral_constant<int, 32>{});
+    }
+}
+
+int slab_of(int64_t states) { return (int)std::min<int64_t>(states, ssb::kSlab); }
+
+int64_t channel_blocks(int64_t per_group, int tl, int warps) {
+    const int64_t cb = (int64_t)warps * 2 * (32 / tl);
+    return (per_group + cb - 1) / cb;
+}
+
+size_t smem_of(bool backward, int tl, int64_t states) {
+    return with_split(tl, [&](auto k) {
+        constexpr int TL = decltype(k)::value;
+        return backward ? ssb::selective_bwd_smem<TL, kBwdWarps>(states, slab_of(states))
+                        : ssb::selective_fwd_smem<TL, kFwdWarps>(states, slab_of(states));
+    });
+}
+
+// Lanes across time: the fewest (they cost shuffles) that give every SM the warps it can hold.
+int split_of(bool backward, int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
+    const int warps = backward ? kBwdWarps : kFwdWarps;
+    const int64_t want = (int64_t)sm_count() * (backward ? 1 : 3);
+    for (int tl = 4; tl < 32; tl *= 2)
+        if (groups * channel_blocks(per_group, tl, warps) * std::max<int64_t>(sequences, 1) >= want &&
+            smem_of(backward, tl, states) <= kSmemLimit)
+            return tl;
+    return 32;
+}
+
+int check_selective(const ssb_selective_t *p, bool data) {
+    if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (int rc = check_sizes(p->dtype, {p->batch, p->channels, p->steps, p->states})) return rc;
+    if (p->states < 1 || p->states > kMaxStates)
+        return fail(SSB_ERR_UNSUPPORTED, "states=%lld: 1 to %lld are supported", (long long)p->states, (long long)kMaxStates);
+    if (p->groups < 1 || p->channels % p->groups != 0)
+        return fail(SSB_ERR_BAD_ARG, "%lld channels do not divide into %lld groups", (long long)p->channels, (long long)p->groups);
+    if (int rc = check_sequences(p->batch, p->sequences, p->offsets, p->lengths)) return rc;
+    if (!data || p->channels == 0) return SSB_OK;
+    if (p->batch > 0 && p->steps > 0) {
+        for (const auto &[v, name] : {std::pair<const ssb_view_t &, const char *>{p->x, "x"}, {p->dt, "dt"}, {p->B, "B"}, {p->C, "C"}})
+            if (int rc = check_data(v.data, p->dtype, name)) return rc;
+        if (!aligned(p->z.data, size_of(p->dtype))) return fail(SSB_ERR_ALIGNMENT, "z is not aligned to its element size");
+    }
+    if (int rc = check_data(p->A, SSB_F32, "A")) return rc;
+    for (const void *f : {(const void *)p->D, (const void *)p->dt_bias, (const void *)p->state, (const void *)p->state_out,
+                          (const void *)p->checkpoints})
+        if (!aligned(f, 4)) return fail(SSB_ERR_ALIGNMENT, "a float32 operand is not aligned to its element size");
+    return SSB_OK;
+}
+
+int64_t count_of(const ssb_selective_t *p) { return p->offsets != nullptr ? p->sequences : p->batch; }
+
+int backward_split(const ssb_selective_t *p) {
+    return split_of(true, p->channels / p->groups, p->groups, count_of(p), p->states);
+}
+int64_t checkpoint_slots(const ssb_selective_t *p) {
+    const int64_t tile = backward_split(p) * ssb::kRun;
+    return p->offsets != nullptr ? p->steps / tile + p->sequences + 1 : p->batch * ((p->steps + tile - 1) / tile);
+}
+
+ssb::SelectiveArgs selective_args(const ssb_selective_t *p, int tl, int warps) {
+    ssb::SelectiveArgs a{};
+    const bool from_zero = p->offsets == nullptr, even = p->groups == 1 || p->channels / p->groups % 2 == 0;
+    a.channels = p->channels;
+    a.groups = p->groups;
+    a.per_group = p->channels / p->groups;
+    a.states = p->states;
+    a.blocks_per_group = (int)channel_blocks(a.per_group, tl, warps);
+    a.softplus = p->softplus;
+    a.slab = slab_of(p->states);
+    a.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
+    a.x = view3(p->x, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    a.dt = view3(p->dt, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    a.z = view3(p->z, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    a.out = view3(p->out, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    a.B = proj_view(p->B, p->batch, p->groups, p->states, p->steps);
+    a.C = proj_view(p->C, p->batch, p->groups, p->states, p->steps);
+    a.A = p->A;
+    a.D = p->D;
+    a.dt_bias = p->dt_bias;
+    a.state = p->state;
+    a.state_out = p->state_out;
+    a.checkpoints = p->checkpoints;
+    if (p->checkpoints != nullptr) {
+        a.checkpoint_slots = checkpoint_slots(p);
+        for (a.tile_log2 = 3; (1 << a.tile_log2) < backward_split(p) * ssb::kRun;) ++a.tile_log2;
+    }
+    return a;
+}
+
+// CTAs that share the sequences of one channel block in the backward: each keeps one set of sums for A, D and dt_bias.
+int64_t backward_rows(const ssb_selective_t *p) {
+    const int64_t blocks = p->groups * channel_blocks(p->channels / p->groups, backward_split(p), kBwdWarps);
+    const int64_t want = std::max<int64_t>(1, (4 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1));
+    return std::max<int64_t>(1, std::min(count_of(p), want));
+}
+
+struct BackwardParts {
+    int64_t proj, A, channel;  // floats of one part
+    int64_t parts_proj, parts_seq;
+    size_t bytes() const { return sizeof(float) * (2 * parts_proj * proj + parts_seq * (A + 2 * channel)); }
+};
+BackwardParts backward_parts(const ssb_selective_t *p) {
+    return {p->batch * p->steps * p->groups * p->states, p->channels * p->states, p->channels,
+            channel_blocks(p->channels / p->groups, backward_split(p), kBwdWarps), backward_rows(p)};
+}
+
+// ---- short convolution ----------------------------------------------------------------------------
+template <typename F>
+int with_width(int64_t width, F &&f) {
+    if (width == 2) return f(std::integral_constant<int, 2>{});
+    if (width == 3) return f(std::integral_constant<int, 3>{});
+    return f(std::integral_constant<int, 4>{});
+}
+int check_width(int64_t width) {
+    return width >= 2 && width <= 4 ? SSB_OK : fail(SSB_ERR_UNSUPPORTED, "width=%lld: 2, 3 and 4 are supported", (long long)width);
+}
+
+int check_conv(const ssb_short_conv_t *p, bool data) {
+    if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (int rc = check_sizes(p->dtype, {p->batch, p->channels, p->steps})) return rc;
+    if (int rc = check_width(p->width)) return rc;
+    if (int rc = check_sequences(p->batch, p->sequences, p->offsets, p->lengths)) return rc;
+    if (!data || p->channels == 0) return SSB_OK;
+    if (p->batch > 0 && p->steps > 0) {
+        if (int rc = check_data(p->x.data, p->dtype, "x")) return rc;
+        if (p->offsets != nullptr && p->x.stride[1] != 1)
+            return fail(SSB_ERR_UNSUPPORTED, "packed sequences need a channels-last view of x");
+    }
+    if (int rc = check_data(p->weight, p->weight_f32 ? SSB_F32 : p->dtype, "weight")) return rc;
+    if (!aligned(p->bias, p->weight_f32 ? 4 : size_of(p->dtype))) return fail(SSB_ERR_ALIGNMENT, "bias is not aligned to its element size");
+    if (!aligned(p->state, size_of(p->dtype)) || !aligned(p->state_out, size_of(p->dtype)))
+        return fail(SSB_ERR_ALIGNMENT, "a state is not aligned to its element size");
+    return SSB_OK;
+}
+
+// Channels-last kernels take any view whose channels are adjacent; with 4 channels per access where all of them allow it.
+struct ConvForm {
+    bool channels_last;
+    int lump;
+    int64_t channel_blocks, chunk_blocks;
+};
+bool lumps(const ssb_view_t &v, int dtype) {
+    return v.stride[1] == 1 && v.stride[0] % 4 == 0 && v.stride[2] % 4 == 0 && aligned(v.data, 4 * size_of(dtype));
+}
+ConvForm conv_form(const ssb_short_conv_t *p, std::initializer_list<const ssb_view_t *> views) {
+    bool cl = true, vec = p->channels % 4 == 0;
+    for (const ssb_view_t *v : views) {
+        cl = cl && v->stride[1] == 1;
+        vec = vec && lumps(*v, p->dtype);
+    }
+    // time adjacent as well (one channel, or one step): the rows kernels do as well, but packed rows need the others
+    ConvForm f{cl, vec ? 4 : 1, 0, 0};
+    const int64_t chunk = cl ? ssb::kConvChunk * ssb::kConvWarps : 4 * 32 * ssb::kRun;
+    f.channel_blocks = cl ? (p->channels + 32 * f.lump - 1) / (32 * f.lump) : (p->channels + ssb::kConvWarps - 1) / ssb::kConvWarps;
+    f.chunk_blocks = std::max<int64_t>(1, (p->steps + chunk - 1) / chunk);
+    return f;
+}
+// Parts of the taps' gradient: the same for either form and lump, so that the query needs no views.
+int64_t conv_parts(const ssb_short_conv_t *p) {
+    const int64_t chunk = ssb::kConvChunk * ssb::kConvWarps;
+    return std::max<int64_t>(1, p->batch) * std::max<int64_t>(1, (p->steps + chunk - 1) / chunk);
+}
+
+ssb::ConvArgs conv_args(const ssb_short_conv_t *p, const ConvForm &f) {
+    ssb::ConvArgs a{};
+    a.channels = p->channels;
+    a.rows = p->batch;
+    a.channel_blocks = f.channel_blocks;
+    a.chunk_blocks = f.chunk_blocks;
+    a.silu = p->silu;
+    a.weight_f32 = p->weight_f32;
+    a.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
+    a.x = view3(p->x, p->dtype, p->batch, p->channels, p->steps, false, false);
+    a.out = view3(p->out, p->dtype, p->batch, p->channels, p->steps, false, false);
+    a.weight = p->weight;
+    a.bias = p->bias;
+    a.state = p->state;
+    a.state_out = p->state_out;
+    return a;
+}
+
+int conv_grid(const ConvForm &f, int64_t rows, unsigned *grid) {
+    const int64_t blocks = f.channel_blocks * f.chunk_blocks * (rows + (f.channels_last ? 1 : 0));
+    if (blocks > 2147483647) return fail(SSB_ERR_UNSUPPORTED, "more than 2^31 blocks");
+    *grid = (unsigned)blocks;
+    return SSB_OK;
+}
+
+int check_step(int dtype, int64_t entries, int64_t channels, int64_t pool, const int32_t *slots) {
+    if (int rc = check_sizes(dtype, {entries, channels, pool})) return rc;
+    if (entries > 2147483647) return fail(SSB_ERR_UNSUPPORTED, "more than 2^31 entries");
+    if (slots == nullptr && pool < entries)
+        return fail(SSB_ERR_BAD_ARG, "%lld entries without slots need as many states, got %lld", (long long)entries, (long long)pool);
+    return SSB_OK;
+}
+
+}  // namespace
+
+namespace ssb_host {
+int take_state_space_status(int word[2]) {
+    cudaError_t e = cudaMemcpyFromSymbol(word, ssb::g_status_word, 2 * sizeof(int));
+    if (e == cudaSuccess && word[0] != 0) {
+        const int zero[2] = {0, 0};
+        e = cudaMemcpyToSymbol(ssb::g_status_word, zero, sizeof(zero));
+    }
+    return (int)e;
+}
+}  // namespace ssb_host
+
+extern "C" {
+
+size_t ssb_selective_checkpoint_bytes(const ssb_selective_t *p) {
+    if (check_selective(p, false) != SSB_OK) return 0;
+    return sizeof(float) * (size_t)(checkpoint_slots(p) * p->states * p->channels);
+}
+
+int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
+    if (int rc = check_selective(p, true)) return rc;
+    const int64_t count = count_of(p);
+    if (p->channels == 0 || count == 0) return SSB_OK;
+    if (p->steps > 0 && p->batch > 0)
+        if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
+    int tl = split_of(false, p->channels / p->groups, p->groups, count, p->states);
+    if (p->checkpoints != nullptr) tl = std::min(tl, backward_split(p));  // checkpoints lie at tile starts
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        return with_split(tl, [&](auto k) {
+            constexpr int TL = decltype(k)::value;
+            const ssb::SelectiveArgs a = selective_args(p, TL, kFwdWarps);
+            auto kernel = ssb::selective_fwd_kernel<io_t, TL, kFwdWarps>;
+            const size_t smem = ssb::selective_fwd_smem<TL, kFwdWarps>(p->states, a.slab);
+            if (int rc = allow_smem(kernel, smem)) return rc;
+            const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)std::min<int64_t>(count, 65535));
+            kernel<<<grid, kFwdWarps * 32, smem, (cudaStream_t)stream>>>(a);
+            return check_launch("selective_fwd_kernel");
+        });
+    });
+}
+
+size_t ssb_selective_bwd_workspace_bytes(const ssb_selective_t *p) {
+    if (check_selective(p, false) != SSB_OK) return 0;
+    return backward_parts(p).bytes();
+}
+
+int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_selective(p, true)) return rc;
+    if (g == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (p->channels == 0) return SSB_OK;
+    const int64_t count = count_of(p);
+    if (p->steps > 0 && p->batch > 0) {
+        for (const auto &[v, name] : {std::pair<const ssb_view_t &, const char *>{g->gout, "gout"}, {g->gx, "gx"}, {g->gdt, "gdt"},
+                                      {g->gB, "gB"}, {g->gC, "gC"}})
+            if (int rc = check_data(v.data, p->dtype, name)) return rc;
+        if (p->z.data != nullptr)
+            if (int rc = check_data(g->gz.data, p->dtype, "gz")) return rc;
+        if (p->checkpoints == nullptr) return fail(SSB_ERR_BAD_ARG, "the backward needs the forward's checkpoints");
+    }
+    if (int rc = check_data(g->gA, SSB_F32, "gA")) return rc;
+    const BackwardParts parts = backward_parts(p);
+    if (workspace == nullptr || workspace_bytes < parts.bytes() || !aligned(workspace, 4))
+        return fail(SSB_ERR_WORKSPACE, "the backward needs %zu bytes of workspace, got %zu", parts.bytes(), workspace_bytes);
+    float *part = static_cast<float *>(workspace);
+    ssb::SelectiveGradArgs q{};
+    const bool from_zero = p->offsets == nullptr, even = p->groups == 1 || p->channels / p->groups % 2 == 0;
+    q.gout = view3(g->gout, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    q.gx = view3(g->gx, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    q.gdt = view3(g->gdt, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    q.gz = view3(g->gz, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
+    q.gstate_out = g->gstate_out;
+    q.gstate = g->gstate;
+    q.part_B = part;
+    q.part_C = q.part_B + parts.parts_proj * parts.proj;
+    q.part_A = q.part_C + parts.parts_proj * parts.proj;
+    q.part_D = q.part_A + parts.parts_seq * parts.A;
+    q.part_bias = q.part_D + parts.parts_seq * parts.channel;
+    q.rows = p->batch;
+    const int rc = with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        return with_split(backward_split(p), [&](auto k) {
+            constexpr int TL = decltype(k)::value;
+            const ssb::SelectiveArgs a = selective_args(p, TL, kBwdWarps);
+            auto kernel = ssb::selective_bwd_kernel<io_t, TL, kBwdWarps>;
+            const size_t smem = ssb::selective_bwd_smem<TL, kBwdWarps>(p->states, a.slab);
+            if (int bad = allow_smem(kernel, smem)) return bad;
+            const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)parts.parts_seq);
+            kernel<<<grid, kBwdWarps * 32, smem, (cudaStream_t)stream>>>(a, q);
+            return check_launch("selective_bwd_kernel");
+        });
+    });
+    if (rc != SSB_OK) return rc;
+    ssb::SelectiveReduceArgs r{};
+    r.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
+    r.rows = p->batch;
+    r.groups = p->groups;
+    r.states = p->states;
+    r.channels = p->channels;
+    r.parts_proj = (int)parts.parts_proj;
+    r.parts_seq = (int)parts.parts_seq;
+    r.part_B = q.part_B;
+    r.part_C = q.part_C;
+    r.part_A = q.part_A;
+    r.part_D = q.part_D;
+    r.part_bias = q.part_bias;
+    r.gB = proj_view(g->gB, p->batch, p->groups, p->states, p->steps);
+    r.gC = proj_view(g->gC, p->batch, p->groups, p->states, p->steps);
+    r.gA = g->gA;
+    r.gD = g->gD;
+    r.gbias = g->gdt_bias;
+    const auto blocks = [](int64_t n, int64_t cap) { return std::min<int64_t>((n + 255) / 256, cap); };
+    r.proj_blocks = count > 0 ? (int)blocks(parts.proj, 16ll * sm_count()) : 0;
+    const int64_t others = blocks(parts.A + 2 * parts.channel, 4ll * sm_count());
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        ssb::selective_reduce_kernel<io_t><<<(unsigned)(r.proj_blocks + others), 256, 0, (cudaStream_t)stream>>>(r);
+        return check_launch("selective_reduce_kernel");
+    });
+}
+
+int ssb_selective_step(const ssb_selective_step_t *p, void *stream) {
+    if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (int rc = check_step(p->dtype, p->entries, p->channels, p->pool, p->slots)) return rc;
+    if (int rc = check_sizes(p->dtype, {std::max(p->entries, p->pool), p->channels, p->states})) return rc;
+    if (p->states < 1 || p->states > kMaxStates)
+        return fail(SSB_ERR_UNSUPPORTED, "states=%lld: 1 to %lld are supported", (long long)p->states, (long long)kMaxStates);
+    if (p->groups < 1 || p->channels % p->groups != 0)
+        return fail(SSB_ERR_BAD_ARG, "%lld channels do not divide into %lld groups", (long long)p->channels, (long long)p->groups);
+    if (p->entries == 0 || p->channels == 0) return SSB_OK;
+    for (const auto &[v, name] : {std::pair<const ssb_view_t &, const char *>{p->x, "x"}, {p->dt, "dt"}, {p->B, "B"}, {p->C, "C"}, {p->out, "out"}})
+        if (int rc = check_data(v.data, p->dtype, name)) return rc;
+    if (!aligned(p->z.data, size_of(p->dtype))) return fail(SSB_ERR_ALIGNMENT, "z is not aligned to its element size");
+    if (int rc = check_data(p->A, SSB_F32, "A")) return rc;
+    if (p->pool > 0)
+        if (int rc = check_data(p->state, SSB_F32, "state")) return rc;
+    if (!aligned(p->D, 4) || !aligned(p->dt_bias, 4)) return fail(SSB_ERR_ALIGNMENT, "a float32 operand is not aligned to its element size");
+    ssb::SelectiveStepArgs a{};
+    a.channels = p->channels;
+    a.per_group = p->channels / p->groups;
+    a.states = p->states;
+    a.softplus = p->softplus;
+    a.vec = p->states % 4 == 0 && aligned(p->state, 16) && aligned(p->A, 16);
+    a.slots = {p->slots, p->entries, p->pool};
+    a.x = view2(p->x, p->entries, p->channels);
+    a.dt = view2(p->dt, p->entries, p->channels);
+    a.z = view2(p->z, p->entries, p->channels);
+    a.out = view2(p->out, p->entries, p->channels);
+    a.B = view2(p->B, p->entries, p->groups, p->states);
+    a.C = view2(p->C, p->entries, p->groups, p->states);
+    a.A = p->A;
+    a.D = p->D;
+    a.dt_bias = p->dt_bias;
+    a.state = p->state;
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        const auto launch = [&](auto kernel, int lanes) {
+            const int64_t blocks = (p->channels + 128 / lanes - 1) / (128 / lanes);
+            if (blocks > 65535) return fail(SSB_ERR_UNSUPPORTED, "too many channels");
+            kernel<<<dim3((unsigned)p->entries, (unsigned)blocks), 128, 0, (cudaStream_t)stream>>>(a);
+            return check_launch("selective_step_kernel");
+        };
+        if (p->states <= 4) return launch(ssb::selective_step_kernel<io_t, 1>, 1);
+        if (p->states <= 8) return launch(ssb::selective_step_kernel<io_t, 2>, 2);
+        if (p->states <= 16) return launch(ssb::selective_step_kernel<io_t, 4>, 4);
+        if (p->states <= 32) return launch(ssb::selective_step_kernel<io_t, 8>, 8);
+        return launch(ssb::selective_step_kernel<io_t, 16>, 16);
+    });
+}
+
+int ssb_short_conv_fwd(const ssb_short_conv_t *p, void *stream) {
+    if (int rc = check_conv(p, true)) return rc;
+    const int64_t count = p->offsets != nullptr ? p->sequences : p->batch;
+    if (p->channels == 0 || count == 0) return SSB_OK;
+    if (p->steps > 0)
+        if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
+    if (p->offsets != nullptr && p->steps > 0 && p->out.stride[1] != 1)
+        return fail(SSB_ERR_UNSUPPORTED, "packed sequences need a channels-last view of out");
+    ConvForm f = conv_form(p, {&p->x, &p->out});
+    if (p->steps == 0) f = {true, 1, (p->channels + 31) / 32, 1};
+    const ssb::ConvArgs a = conv_args(p, f);
+    unsigned grid = 0;
+    if (int rc = conv_grid(f, p->batch, &grid)) return rc;
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        return with_width(p->width, [&](auto k) {
+            constexpr int W = decltype(k)::value;
+            const int threads = ssb::kConvWarps * 32;
+            if (!f.channels_last) ssb::conv_rows_fwd_kernel<io_t, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+            else if (f.lump == 4) ssb::conv_cl_fwd_kernel<io_t, 4, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+            else ssb::conv_cl_fwd_kernel<io_t, 1, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a);
+            return check_launch("short convolution");
+        });
+    });
+}
+
+size_t ssb_short_conv_bwd_workspace_bytes(const ssb_short_conv_t *p) {
+    if (check_conv(p, false) != SSB_OK) return 0;
+    return sizeof(float) * (size_t)(conv_parts(p) * p->channels * (p->width + 1));
+}
+
+int ssb_short_conv_bwd(const ssb_short_conv_t *p, const ssb_short_conv_grads_t *g, void *workspace, size_t workspace_bytes, void *stream) {
+    if (int rc = check_conv(p, true)) return rc;
+    if (g == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (p->channels == 0) return SSB_OK;
+    if (p->steps > 0 && p->batch > 0) {
+        if (int rc = check_data(g->gout.data, p->dtype, "gout")) return rc;
+        if (int rc = check_data(g->gx.data, p->dtype, "gx")) return rc;
+        if (p->offsets != nullptr && (g->gout.stride[1] != 1 || g->gx.stride[1] != 1))
+            return fail(SSB_ERR_UNSUPPORTED, "packed sequences need channels-last views");
+    }
+    const int weight_type = p->weight_f32 ? SSB_F32 : p->dtype;
+    if (int rc = check_data(g->gweight, weight_type, "gweight")) return rc;
+    if (!aligned(g->gbias, size_of(weight_type)) || !aligned(g->gstate, size_of(p->dtype)) || !aligned(g->gstate_out, size_of(p->dtype)))
+        return fail(SSB_ERR_ALIGNMENT, "a gradient is not aligned to its element size");
+    const size_t need = ssb_short_conv_bwd_workspace_bytes(p);
+    if (workspace == nullptr || workspace_bytes < need || !aligned(workspace, 4))
+        return fail(SSB_ERR_WORKSPACE, "the backward needs %zu bytes of workspace, got %zu", need, workspace_bytes);
+    ConvForm f = conv_form(p, {&p->x, &g->gout, &g->gx});
+    if (p->steps == 0) f = {true, 1, (p->channels + 31) / 32, 1};
+    const ssb::ConvArgs a = conv_args(p, f);
+    ssb::ConvGradArgs q{};
+    q.gout = view3(g->gout, p->dtype, p->batch, p->channels, p->steps, false, false);
+    q.gx = view3(g->gx, p->dtype, p->batch, p->channels, p->steps, false, false);
+    q.gstate_out = g->gstate_out;
+    q.gstate = g->gstate;
+    q.part = static_cast<float *>(workspace);
+    unsigned grid = 0;
+    if (int rc = conv_grid(f, p->batch, &grid)) return rc;
+    const int64_t parts = p->batch * f.chunk_blocks;
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        const int rc = with_width(p->width, [&](auto k) {
+            constexpr int W = decltype(k)::value;
+            const int threads = ssb::kConvWarps * 32;
+            if (grid == 0) return (int)SSB_OK;
+            if (!f.channels_last) ssb::conv_rows_bwd_kernel<io_t, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a, q);
+            else if (f.lump == 4) ssb::conv_cl_bwd_kernel<io_t, 4, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a, q);
+            else ssb::conv_cl_bwd_kernel<io_t, 1, W><<<grid, threads, 0, (cudaStream_t)stream>>>(a, q);
+            return check_launch("short convolution backward");
+        });
+        if (rc != SSB_OK) return rc;
+        const int64_t blocks = std::min<int64_t>((p->channels * (p->width + 1) + 255) / 256, 8ll * sm_count());
+        ssb::conv_reduce_kernel<io_t><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(q.part, parts, p->channels, (int)p->width,
+                                                                                          p->weight_f32, g->gweight, g->gbias);
+        return check_launch("conv_reduce_kernel");
+    });
+}
+
+int ssb_short_conv_step(const ssb_short_conv_step_t *p, void *stream) {
+    if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
+    if (int rc = check_step(p->dtype, p->entries, p->channels, p->pool, p->slots)) return rc;
+    if (int rc = check_width(p->width)) return rc;
+    if (p->entries == 0 || p->channels == 0) return SSB_OK;
+    if (int rc = check_data(p->x.data, p->dtype, "x")) return rc;
+    if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
+    if (int rc = check_data(p->weight, p->weight_f32 ? SSB_F32 : p->dtype, "weight")) return rc;
+    if (!aligned(p->bias, p->weight_f32 ? 4 : size_of(p->dtype))) return fail(SSB_ERR_ALIGNMENT, "bias is not aligned to its element size");
+    if (p->pool > 0)
+        if (int rc = check_data(p->state, p->dtype, "state")) return rc;
+    ssb::ConvStepArgs a{};
+    a.channels = p->channels;
+    a.width = (int)p->width;
+    a.silu = p->silu;
+    a.weight_f32 = p->weight_f32;
+    a.slots = {p->slots, p->entries, p->pool};
+    a.x = view2(p->x, p->entries, p->channels);
+    a.out = view2(p->out, p->entries, p->channels);
+    a.weight = p->weight;
+    a.bias = p->bias;
+    a.state = p->state;
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        return with_width(p->width, [&](auto k) {
+            constexpr int W = decltype(k)::value;
+            const int64_t blocks = (p->channels + 127) / 128;
+            if (blocks > 65535) return fail(SSB_ERR_UNSUPPORTED, "too many channels");
+            ssb::conv_step_kernel<io_t, W><<<dim3((unsigned)p->entries, (unsigned)blocks), 128, 0, (cudaStream_t)stream>>>(a);
+            return check_launch("conv_step_kernel");
+        });
+    });
+}
+
+}  // extern "C"

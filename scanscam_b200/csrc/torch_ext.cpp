@@ -11,6 +11,11 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <string>
+#include <tuple>
+#include <vector>
+
 #include "../../include/scanscam_b200.h"
 
 namespace {
@@ -453,6 +458,9 @@ void shard_carry(torch::Tensor aggs, int64_t shard, bool reverse, torch::Tensor 
              "shard_carry");
 }
 
+// ---- state-space operators (not in the reference) --------------------------------------------
+#include "torch_state_space.h"
+
 int64_t device_status() {
     int detail = 0;
     return ssb_device_status(&detail);
@@ -487,5 +495,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("shard_map_backward", &shard_map_backward, "Map (A, D) of the reverse recurrence, walked from the shard's start until |A| <= cut",
           py::arg("gate"), py::arg("outGrad"), py::arg("agg"), py::arg("cut") = 0.0, py::arg("walked") = py::none());
     m.def("shard_carry", &shard_carry, "Fold gathered shard aggregates into the carry entering one shard");
+    m.def("selective_forward", &selective_forward, "Selective state-space scan: (out, state out, checkpoints)",
+          py::call_guard<py::gil_scoped_release>());
+    m.def("selective_backward", &selective_backward, "Gradients of the selective scan", py::call_guard<py::gil_scoped_release>());
+    m.def("selective_step", &selective_step, "One step of the selective scan per entry, states updated in place");
+    m.def("short_conv_forward", &short_conv_forward, "Short causal convolution: (out, window out)",
+          py::call_guard<py::gil_scoped_release>());
+    m.def("short_conv_backward", &short_conv_backward, "Gradients of the short causal convolution",
+          py::call_guard<py::gil_scoped_release>());
+    m.def("short_conv_step", &short_conv_step, "One step of the short convolution per entry, windows updated in place");
     m.def("device_status", &device_status, "Synchronise and return/clear the device-side status code");
 }
