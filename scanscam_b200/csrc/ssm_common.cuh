@@ -132,61 +132,100 @@ __device__ __forceinline__ void store_one(io_t *base, int64_t at, int64_t extent
 
 constexpr int kRun = 8;  // steps a thread holds of each of its two channels
 
-// Steps t .. t+7 of channels c, c+1 of row n as pairs; what lies behind `steps` steps or
-// `channels` channels is zero and is not read.
+// Steps t .. t+7 of channels c, c+1 of row n, as they lie in memory: fetched ahead of their use, opened
+// into pairs when they are needed.  What lies behind `steps` steps or `channels` channels is zero and
+// is not read.
 template <typename io_t>
-__device__ __forceinline__ void load_run(const View3 &v, int64_t n, int64_t c, int64_t t, int steps, int channels,
-                                         int site, pair_t (&r)[kRun]) {
+struct RawRun {
+    static constexpr int kWords = kRun * 2 * (int)sizeof(io_t) / 4;
+    uint32_t w[kWords];
+    bool by_channel;  // words hold 8 steps of one channel, then of the other; else the pair of one step after the other
+};
+
+template <typename io_t>
+__device__ __forceinline__ void fetch_run(const View3 &v, int64_t n, int64_t c, int64_t t, int steps, int channels, int site,
+                                          RawRun<io_t> &r) {
     const io_t *base = static_cast<const io_t *>(v.data);
     const int64_t at = n * v.sn + c * v.sc + t * v.st;
 #pragma unroll
-    for (int k = 0; k < kRun; ++k) r[k] = 0;
+    for (int k = 0; k < RawRun<io_t>::kWords; ++k) r.w[k] = 0;
+    r.by_channel = false;
     if (v.access == kPairs && channels == 2) {
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
             const int64_t i = at + k * v.st;
             if (k < steps && SSB_VECTOR_OK(base + i, 2 * (int)sizeof(io_t), i + 1, v.extent, site)) {
                 if constexpr (sizeof(io_t) == 2) {
-                    float lo, hi;
-                    unpack2<io_t>(*reinterpret_cast<const uint32_t *>(base + i), lo, hi);
-                    r[k] = make_pair(lo, hi);
+                    r.w[k] = *reinterpret_cast<const uint32_t *>(base + i);
                 } else {
-                    r[k] = *reinterpret_cast<const pair_t *>(base + i);
+                    const uint2 q = *reinterpret_cast<const uint2 *>(base + i);
+                    r.w[2 * k] = q.x;
+                    r.w[2 * k + 1] = q.y;
                 }
             }
         }
     } else if (v.access == kRuns && channels == 2 && steps == kRun) {
-        float f[2][kRun];
+        r.by_channel = true;
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
             const int64_t i = at + q * v.sc;
-            if (!SSB_VECTOR_OK(base + i, 16, i + kRun - 1, v.extent, site)) {
+            if (!SSB_VECTOR_OK(base + i, 16, i + kRun - 1, v.extent, site)) continue;
 #pragma unroll
-                for (int k = 0; k < kRun; ++k) f[q][k] = 0.0f;
-            } else if constexpr (sizeof(io_t) == 2) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(base + i);
-                unpack2<io_t>(w.x, f[q][0], f[q][1]);
-                unpack2<io_t>(w.y, f[q][2], f[q][3]);
-                unpack2<io_t>(w.z, f[q][4], f[q][5]);
-                unpack2<io_t>(w.w, f[q][6], f[q][7]);
-            } else {
-                const float4 a = *reinterpret_cast<const float4 *>(base + i), b = *reinterpret_cast<const float4 *>(base + i + 4);
-                f[q][0] = a.x; f[q][1] = a.y; f[q][2] = a.z; f[q][3] = a.w;
-                f[q][4] = b.x; f[q][5] = b.y; f[q][6] = b.z; f[q][7] = b.w;
+            for (int k = 0; k < RawRun<io_t>::kWords / 8; ++k) {
+                const uint4 f = reinterpret_cast<const uint4 *>(base + i)[k];
+                uint32_t *w = r.w + q * (RawRun<io_t>::kWords / 2) + 4 * k;
+                w[0] = f.x; w[1] = f.y; w[2] = f.z; w[3] = f.w;
             }
         }
-#pragma unroll
-        for (int k = 0; k < kRun; ++k) r[k] = make_pair(f[0][k], f[1][k]);
     } else {
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            float f[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int q = 0; q < 2; ++q)
-                if (k < steps && q < channels) f[q] = load_one<io_t>(base, at + k * v.st + q * v.sc, v.extent, site);
-            r[k] = make_pair(f[0], f[1]);
+            for (int q = 0; q < 2; ++q) {
+                const int64_t i = at + k * v.st + q * v.sc;
+                if (k < steps && q < channels && SSB_INDEX_OK(i, v.extent, site)) {
+                    if constexpr (sizeof(io_t) == 2) r.w[k] |= (uint32_t)reinterpret_cast<const uint16_t *>(base)[i] << (16 * q);
+                    else r.w[2 * k + q] = reinterpret_cast<const uint32_t *>(base)[i];
+                }
+            }
         }
     }
+}
+
+template <typename io_t>
+__device__ __forceinline__ void open_run(const RawRun<io_t> &raw, pair_t (&r)[kRun]) {
+    if constexpr (sizeof(io_t) == 2) {
+        if (raw.by_channel) {
+#pragma unroll
+            for (int k = 0; k < kRun / 2; ++k) {
+                float a, b, c, d;
+                unpack2<io_t>(raw.w[k], a, b);
+                unpack2<io_t>(raw.w[kRun / 2 + k], c, d);
+                r[2 * k] = make_pair(a, c);
+                r[2 * k + 1] = make_pair(b, d);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                float a, b;
+                unpack2<io_t>(raw.w[k], a, b);
+                r[k] = make_pair(a, b);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+            r[k] = raw.by_channel ? make_pair(__uint_as_float(raw.w[k]), __uint_as_float(raw.w[kRun + k]))
+                                  : make_pair(__uint_as_float(raw.w[2 * k]), __uint_as_float(raw.w[2 * k + 1]));
+    }
+}
+
+template <typename io_t>
+__device__ __forceinline__ void load_run(const View3 &v, int64_t n, int64_t c, int64_t t, int steps, int channels,
+                                         int site, pair_t (&r)[kRun]) {
+    RawRun<io_t> raw;
+    fetch_run(v, n, c, t, steps, channels, site, raw);
+    open_run(raw, r);
 }
 
 template <typename io_t>

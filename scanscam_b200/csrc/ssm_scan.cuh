@@ -23,11 +23,12 @@ namespace ssb {
 struct ProjView {  // B or C: [N, G, S, T]
     void *data;
     int64_t sn, sg, ss, st, extent;
+    int access;  // ProjAccess
 };
 
 struct SelectiveArgs {
     int64_t channels, per_group, groups, states;
-    int blocks_per_group, softplus, slab, tile_log2;  // slab: states staged at a time; tile_log2: steps between checkpoints
+    int blocks_per_group, softplus, tile_log2;  // tile_log2: steps between checkpoints
     Sequences seq;
     View3 x, dt, z, out;
     ProjView B, C;
@@ -55,25 +56,95 @@ __device__ __forceinline__ int64_t checkpoint_base(const SelectiveArgs &p, int64
     return p.seq.offsets != nullptr ? (start >> p.tile_log2) + s : s * per_row;
 }
 
-// Steps [t, t + tile) of states [n0, n0 + count) of B or C into shared memory, [state][step]; zero behind `steps`.
-template <typename io_t, int TILE>
-__device__ __forceinline__ void stage_projection(const ProjView &v, int64_t row, int64_t g, int n0, int count, int64_t t,
-                                                 int64_t steps, float *smem) {
-    const io_t *base = static_cast<const io_t *>(v.data);
-    const int64_t at = row * v.sn + g * v.sg + n0 * v.ss + t * v.st;
-    const int total = count * TILE;
-    for (int i = threadIdx.x; i < total; i += blockDim.x) {
-        int n, k;  // the index that is adjacent in memory runs over the lanes
-        if (v.ss == 1) {
-            k = i / count;
-            n = i - k * count;
-        } else {
-            n = i / TILE;
-            k = i % TILE;
-        }
-        smem[n * scan_pad(TILE) + k] = k < steps ? load_one<io_t>(base, at + n * v.ss + k * v.st, v.extent, 210) : 0.0f;
-    }
+// How B and C are fetched: 16 bytes along the states of a step or along the steps of a state where
+// the strides allow it, else element by element.
+enum ProjAccess : int { kProjAny = 0, kProjStates = 1, kProjSteps = 2 };
+
+// States staged at a time: so many that a thread fetches at most two 16-byte pieces of each of B and C.
+template <typename io_t, int TILE, int THREADS>
+__host__ __device__ constexpr int slab_states() {
+    const int n = 2 * THREADS * (16 / (int)sizeof(io_t)) / TILE;
+    return n > kSlab ? kSlab : n;
 }
+
+// One slab's pieces, fetched ahead and put down as fp32 [state][step] when the tile before is done.
+template <typename io_t, int TILE, int THREADS>
+struct ProjPieces {
+    static constexpr int kPer = 16 / (int)sizeof(io_t);  // elements of a piece
+    static constexpr int kSlabStates = slab_states<io_t, TILE, THREADS>();
+    static constexpr int kPieces = (kSlabStates * TILE / kPer + THREADS - 1) / THREADS;
+    uint4 piece[kPieces];
+
+    // Steps [t, t + TILE) of states [n0, n0 + count); zero behind `steps` steps.
+    __device__ __forceinline__ void fetch(const ProjView &v, int64_t row, int64_t g, int n0, int count, int64_t t, int64_t steps) {
+        if (v.access == kProjAny) return;
+        const io_t *base = static_cast<const io_t *>(v.data);
+        const int64_t at = row * v.sn + g * v.sg + n0 * v.ss + t * v.st;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int i = threadIdx.x + j * THREADS;
+            // along the states: lanes hold neighbouring steps, so that the fp32 stores below meet no bank twice
+            const int n = v.access == kProjStates ? i / TILE * kPer : i / (TILE / kPer);
+            const int k = v.access == kProjStates ? i % TILE : i % (TILE / kPer) * kPer;
+            piece[j] = make_uint4(0, 0, 0, 0);
+            const int64_t e = at + n * v.ss + k * v.st;
+            if (n < count && k < steps && SSB_VECTOR_OK(base + e, 16, e + kPer - 1, v.extent, 210))
+                piece[j] = *reinterpret_cast<const uint4 *>(base + e);
+        }
+    }
+    __device__ __forceinline__ void put(const ProjView &v, int64_t row, int64_t g, int n0, int count, int64_t t, int64_t steps,
+                                        float *smem) const {
+        if (v.access == kProjAny) {
+            const io_t *base = static_cast<const io_t *>(v.data);
+            const int64_t at = row * v.sn + g * v.sg + n0 * v.ss + t * v.st;
+            const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+            // the lanes run along whichever index is adjacent in memory
+            const bool by_state = v.ss <= v.st;
+            const int outer = by_state ? TILE : count, inner = by_state ? count : TILE;
+            for (int o = warp; o < outer; o += THREADS / 32)
+                for (int i = lane; i < inner; i += 32) {
+                    const int n = by_state ? i : o, k = by_state ? o : i;
+                    smem[n * scan_pad(TILE) + k] = k < steps ? load_one<io_t>(base, at + n * v.ss + k * v.st, v.extent, 210) : 0.0f;
+                }
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const int i = threadIdx.x + j * THREADS;
+            float f[kPer];
+            if constexpr (sizeof(io_t) == 2) {
+                unpack2<io_t>(piece[j].x, f[0], f[1]);
+                unpack2<io_t>(piece[j].y, f[2], f[3]);
+                unpack2<io_t>(piece[j].z, f[4], f[5]);
+                unpack2<io_t>(piece[j].w, f[6], f[7]);
+            } else {
+                f[0] = __uint_as_float(piece[j].x); f[1] = __uint_as_float(piece[j].y);
+                f[2] = __uint_as_float(piece[j].z); f[3] = __uint_as_float(piece[j].w);
+            }
+            if (v.access == kProjStates) {
+                const int n = i / TILE * kPer, k = i % TILE;
+                if (n < count) {
+#pragma unroll
+                    for (int e = 0; e < kPer; ++e) smem[(n + e) * scan_pad(TILE) + k] = f[e];
+                }
+            } else {
+                const int n = i / (TILE / kPer), k = i % (TILE / kPer) * kPer;
+                if (n < count) {
+#pragma unroll
+                    for (int e = 0; e < kPer; e += 4) {
+                        // a fetched piece may reach behind the last step: those elements are not the sequence's
+                        float4 q = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                        if (k + e + 0 >= steps) q.x = 0.0f;
+                        if (k + e + 1 >= steps) q.y = 0.0f;
+                        if (k + e + 2 >= steps) q.z = 0.0f;
+                        if (k + e + 3 >= steps) q.w = 0.0f;
+                        *reinterpret_cast<float4 *>(smem + n * scan_pad(TILE) + k + e) = q;
+                    }
+                }
+            }
+        }
+    }
+};
 
 // A[c, n] * log2(e) of the CTA's channels, [state][channel]; zero behind the last channel.  An
 // infinite entry becomes the largest finite one: with a step of zero it then decays by 2^0 = 1, as
@@ -209,19 +280,100 @@ struct ScanShape {
     static constexpr int PAD = scan_pad(TILE);
 };
 
-template <int TL, int W>
-__host__ __device__ constexpr size_t selective_fwd_smem(int64_t states, int slab) {
-    using H = ScanShape<TL, W>;
-    return sizeof(float) * ((size_t)states * H::CB + (size_t)slab * (H::CB + 2 * H::PAD));
-}
+#ifndef KATONCE
+#define KATONCE 2
+#endif
+constexpr int kAtOnce = KATONCE;
+// Rounds a number of states up to whole pairs: two states are worked on at a time.
+__host__ __device__ constexpr int64_t even_states(int64_t states) { return (states + 1) & ~(int64_t)1; }
 
 template <typename io_t, int TL, int W>
-__global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
+__host__ __device__ constexpr size_t selective_fwd_smem(int64_t states) {
     using H = ScanShape<TL, W>;
+    constexpr int slab = slab_states<io_t, H::TILE, W * 32>();
+    const int64_t even = even_states(states), rows = even < slab ? even : slab;
+    return sizeof(float) * (size_t)(2 * even * H::CB + 2 * rows * H::PAD);
+}
+
+// One tile's states [0, count) of the slab, two at a time: their chains are independent, and hide
+// each other's latency.  `decay` and `carry` start at the slab's first state.
+template <int TL, int W>
+__device__ __forceinline__ void scan_states(const float *decay, float *carry, const float *Bs, const float *Cs, int count, int tl, int cl,
+                                            const pair_t (&dt)[kRun], const pair_t (&u)[kRun], pair_t (&y)[kRun]) {
+    using H = ScanShape<TL, W>;
+#pragma unroll 1
+    for (int n = 0; n < count; n += kAtOnce) {
+        pair_t a[kAtOnce][kRun], b[kAtOnce][kRun], P[kAtOnce], F[kAtOnce], h[kAtOnce], h_in[kAtOnce];
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+            const pair_t A = *reinterpret_cast<const pair_t *>(decay + (n + q) * H::CB + cl);
+            h_in[q] = *reinterpret_cast<const pair_t *>(carry + (n + q) * H::CB + cl);
+            float v[kRun];
+            load8(Bs + (n + q) * H::PAD + tl * kRun, v);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                a[q][k] = exp2_pair(mul2(dt[k], A));
+                b[q][k] = mul2(u[k], both(v[k]));
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+            P[q] = a[q][0];
+            F[q] = b[q][0];
+        }
+#pragma unroll
+        for (int k = 1; k < kRun; ++k) {
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) {
+                F[q] = fma2(a[q][k], F[q], b[q][k]);
+                P[q] = mul2(P[q], a[q][k]);
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < TL; d <<= 1) {
+#pragma unroll
+            for (int q = 0; q < kAtOnce; ++q) {
+                const pair_t P0 = shfl_up2(P[q], d * H::DL), F0 = shfl_up2(F[q], d * H::DL);
+                if (tl >= d) {
+                    F[q] = fma2(P[q], F0, F[q]);
+                    P[q] = mul2(P[q], P0);
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+            const pair_t h_end = fma2(P[q], h_in[q], F[q]);  // the state behind this lane's steps
+            h[q] = shfl_up2(h_end, H::DL);
+            if (tl == 0) h[q] = h_in[q];
+            __syncwarp();  // all lanes have read what is replaced
+            if (tl == TL - 1) *reinterpret_cast<pair_t *>(carry + (n + q) * H::CB + cl) = h_end;
+        }
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+            float v[kRun];
+            load8(Cs + (n + q) * H::PAD + tl * kRun, v);
+#pragma unroll
+            for (int k = 0; k < kRun; ++k) {
+                h[q] = fma2(a[q][k], h[q], b[q][k]);
+                y[k] = fma2(h[q], both(v[k]), y[k]);
+            }
+        }
+    }
+}
+
+#ifndef FWD_MINB
+#define FWD_MINB 2
+#endif
+template <typename io_t, int TL, int W>
+__global__ void __launch_bounds__(W * 32, (W == 4 ? FWD_MINB : (FWD_MINB + 1) / 2)) selective_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
+    using H = ScanShape<TL, W>;
+    using Pieces = ProjPieces<io_t, H::TILE, W * 32>;
     extern __shared__ __align__(16) float smem[];
-    float *carry = smem;                                   // [states][CB]: the state entering the tile
-    float *decay = carry + p.states * H::CB;               // [slab][CB]
-    float *Bs = decay + p.slab * H::CB, *Cs = Bs + p.slab * H::PAD;
+    const int S = (int)p.states, even = (int)even_states(S);
+    const int slab = even < Pieces::kSlabStates ? even : Pieces::kSlabStates;  // even: an odd last state has a partner of zeros
+    float *carry = smem;                     // [even][CB]: the state entering the tile
+    float *decay = carry + even * H::CB;     // [even][CB]
+    float *Bs = decay + even * H::CB, *Cs = Bs + slab * H::PAD;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tl = lane / H::DL, cl = warp * H::CW + 2 * (lane % H::DL);
     const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
@@ -229,7 +381,6 @@ __global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_cons
     const int64_t c_end = c0 + H::CB < (g + 1) * p.per_group ? c0 + H::CB : (g + 1) * p.per_group;
     const int64_t c = c0 + cl;
     const int nc = c_end - c >= 2 ? 2 : (c_end > c ? 1 : 0);  // channels of this thread that exist
-    const int S = (int)p.states;
     float2 D = make_float2(0.0f, 0.0f), bias = D;
     if (p.D != nullptr) {
         if (nc > 0) D.x = load_one(p.D, c, p.channels, 212);
@@ -239,21 +390,39 @@ __global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_cons
         if (nc > 0) bias.x = load_one(p.dt_bias, c, p.channels, 213);
         if (nc > 1) bias.y = load_one(p.dt_bias, c + 1, p.channels, 213);
     }
-    if (S <= p.slab) {  // staged once for all tiles
-        stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
-    }
+    stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
+    if (even != S)  // the partner of an odd last state: decay 1, no input, no read-out
+        for (int i = threadIdx.x; i < H::CB; i += W * 32) decay[S * H::CB + i] = 0.0f;
 
     for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
         const Span sp = span_of(p.seq, s);
         load_states<H::CB, H::CW>(p.state, s, p, c0, c_end, warp, lane, 214, carry);
+        if (even != S && tl == 0) *reinterpret_cast<pair_t *>(carry + S * H::CB + cl) = 0;
         const int64_t slot0 = p.checkpoints != nullptr ? checkpoint_base(p, s, sp.start) : 0;
+        RawRun<io_t> raw_x, raw_dt;
+        Pieces next_B, next_C;
+        const auto fetch = [&](int64_t t0) {  // this thread's runs of the tile at t0
+            const int64_t left = sp.length - t0 - tl * kRun;
+            const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
+            fetch_run(p.x, sp.row, c, sp.start + t0 + tl * kRun, steps, nc, 215, raw_x);
+            fetch_run(p.dt, sp.row, c, sp.start + t0 + tl * kRun, steps, nc, 216, raw_dt);
+        };
+        const auto fetch_projections = [&](int64_t t0, int n0) {
+            const int count = S - n0 < slab ? S - n0 : slab;
+            next_B.fetch(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
+            next_C.fetch(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
+        };
+        if (sp.length > 0) {
+            fetch(0);
+            fetch_projections(0, 0);
+        }
         for (int64_t t0 = 0; t0 < sp.length; t0 += H::TILE) {
             const int64_t left = sp.length - t0 - tl * kRun;
             const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
             const int64_t t = sp.start + t0 + tl * kRun;
             pair_t dt[kRun], u[kRun], y[kRun];
-            load_run<io_t>(p.x, sp.row, c, t, steps, nc, 215, u);
-            load_run<io_t>(p.dt, sp.row, c, t, steps, nc, 216, dt);
+            open_run(raw_x, u);
+            open_run(raw_dt, dt);
             make_steps(dt, bias, p.softplus, steps);
             const pair_t Dp = make_pair(D.x, D.y);
 #pragma unroll
@@ -271,44 +440,22 @@ __global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_cons
                 }
                 __syncwarp();
             }
-            for (int n0 = 0; n0 < S; n0 += p.slab) {
-                const int count = S - n0 < p.slab ? S - n0 : p.slab;
+            for (int n0 = 0; n0 < S; n0 += slab) {
+                const int count = S - n0 < slab ? S - n0 : slab;
                 __syncthreads();
-                if (S > p.slab) stage_decays<H::CB>(p, c0, c_end, n0, count, decay);
-                stage_projection<io_t, H::TILE>(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
-                stage_projection<io_t, H::TILE>(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
+                next_B.put(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
+                next_C.put(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
+                if (count & 1)
+                    for (int i = threadIdx.x; i < H::PAD; i += W * 32) Bs[count * H::PAD + i] = Cs[count * H::PAD + i] = 0.0f;
                 __syncthreads();
-                for (int n = 0; n < count; ++n) {
-                    const pair_t A = *reinterpret_cast<const pair_t *>(decay + n * H::CB + cl);
-                    pair_t *held = reinterpret_cast<pair_t *>(carry + (n0 + n) * H::CB + cl);
-                    const pair_t h_in = *held;
-                    pair_t a[kRun], b[kRun];
-                    float v[kRun];
-                    load8(Bs + n * H::PAD + tl * kRun, v);
-#pragma unroll
-                    for (int k = 0; k < kRun; ++k) {
-                        a[k] = exp2_pair(mul2(dt[k], A));
-                        b[k] = mul2(u[k], both(v[k]));
-                    }
-                    pair_t P = a[0], F = b[0];
-#pragma unroll
-                    for (int k = 1; k < kRun; ++k) {
-                        F = fma2(a[k], F, b[k]);
-                        P = mul2(P, a[k]);
-                    }
-                    compose_left<TL>(P, F, tl);
-                    const pair_t h_end = fma2(P, h_in, F);  // the state behind this lane's steps
-                    pair_t h = shfl_up2(h_end, H::DL);
-                    if (tl == 0) h = h_in;
-                    __syncwarp();
-                    if (tl == TL - 1) *held = h_end;
-                    load8(Cs + n * H::PAD + tl * kRun, v);
-#pragma unroll
-                    for (int k = 0; k < kRun; ++k) {
-                        h = fma2(a[k], h, b[k]);
-                        y[k] = fma2(h, both(v[k]), y[k]);
-                    }
+                // what the next slab needs is under way while this one is worked on
+                if (n0 + slab < S) {
+                    fetch_projections(t0, n0 + slab);
+                } else if (t0 + H::TILE < sp.length) {
+                    fetch(t0 + H::TILE);
+                    fetch_projections(t0 + H::TILE, 0);
                 }
+                scan_states<TL, W>(decay + n0 * H::CB, carry + n0 * H::CB, Bs, Cs, count, tl, cl, dt, u, y);
             }
             __syncwarp();
             if (p.z.data != nullptr) {
@@ -338,23 +485,27 @@ __global__ void __launch_bounds__(W * 32) selective_fwd_kernel(const __grid_cons
 // over the warps of the CTA in shared memory, over CTAs by selective_reduce_kernel in a fixed order.  The warps of
 // a CTA work on different states at a time (warp w on state (i + w) mod count), with a barrier per
 // state, so that none adds to a row of sums that another is adding to, and the order of the additions is always the same.
-template <int TL, int W>
-__host__ __device__ constexpr size_t selective_bwd_smem(int64_t states, int slab) {
+template <typename io_t, int TL, int W>
+__host__ __device__ constexpr size_t selective_bwd_smem(int64_t states) {
     using H = ScanShape<TL, W>;
-    return sizeof(float) * ((size_t)states * H::CB * 2 + (size_t)slab * (2 * H::CB + 4 * H::PAD));
+    constexpr int most = slab_states<io_t, H::TILE, W * 32>();
+    const int64_t slab = states < most ? states : most;
+    return sizeof(float) * (size_t)(states * H::CB * 2 + slab * (2 * H::CB + 4 * H::PAD));
 }
 
 template <typename io_t, int TL, int W>
 __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_constant__ SelectiveArgs p,
                                                               const __grid_constant__ SelectiveGradArgs q) {
     using H = ScanShape<TL, W>;
+    using Pieces = ProjPieces<io_t, H::TILE, W * 32>;
     extern __shared__ __align__(16) float smem[];
+    const int S = (int)p.states, slab = S < Pieces::kSlabStates ? S : Pieces::kSlabStates;
     float *adjoint = smem;                              // [states][CB]: r entering the tile from the right
-    float *gA = adjoint + p.states * H::CB;             // [states][CB]: sums over this CTA's steps
-    float *decay = gA + p.states * H::CB;               // [slab][CB]
-    float *first = decay + p.slab * H::CB;              // [slab][CB]: the state entering the tile
-    float *Bs = first + p.slab * H::CB, *Cs = Bs + p.slab * H::PAD;
-    float *sumB = Cs + p.slab * H::PAD, *sumC = sumB + p.slab * H::PAD;
+    float *gA = adjoint + S * H::CB;                    // [states][CB]: sums over this CTA's steps
+    float *decay = gA + S * H::CB;                      // [slab][CB]
+    float *first = decay + slab * H::CB;                // [slab][CB]: the state entering the tile
+    float *Bs = first + slab * H::CB, *Cs = Bs + slab * H::PAD;
+    float *sumB = Cs + slab * H::PAD, *sumC = sumB + slab * H::PAD;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int tl = lane / H::DL, dl = lane % H::DL, cl = warp * H::CW + 2 * dl;
     const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
@@ -362,7 +513,6 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
     const int64_t c_end = c0 + H::CB < (g + 1) * p.per_group ? c0 + H::CB : (g + 1) * p.per_group;
     const int64_t c = c0 + cl;
     const int nc = c_end - c >= 2 ? 2 : (c_end > c ? 1 : 0);
-    const int S = (int)p.states;
     float2 D = make_float2(0.0f, 0.0f), bias = D;
     if (p.D != nullptr) {
         if (nc > 0) D.x = load_one(p.D, c, p.channels, 230);
@@ -374,7 +524,7 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
     }
     const pair_t Dp = make_pair(D.x, D.y);
     for (int i = threadIdx.x; i < S * H::CB; i += blockDim.x) gA[i] = 0.0f;
-    if (S <= p.slab) stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
+    if (S <= slab) stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
     pair_t gD = 0, gbias = 0;
 
     for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
@@ -389,17 +539,22 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
             const int64_t t = sp.start + t0 + tl * kRun;
             pair_t dt[kRun], u[kRun], gy[kRun], y[kRun];
             pair_t through[kRun], bydecay[kRun];  // sum_n dh B  and  sum_n dh (a h_{t-1}) A log2(e)
-            load_run<io_t>(q.gout, sp.row, c, t, steps, nc, 233, gy);
+            RawRun<io_t> raw_x, raw_dt, raw_z, raw_g;  // all under way before the first is used
+            fetch_run(q.gout, sp.row, c, t, steps, nc, 233, raw_g);
+            if (p.z.data != nullptr) fetch_run(p.z, sp.row, c, t, steps, nc, 234, raw_z);
+            fetch_run(p.x, sp.row, c, t, steps, nc, 235, raw_x);
+            fetch_run(p.dt, sp.row, c, t, steps, nc, 236, raw_dt);
+            open_run(raw_g, gy);
             if (p.z.data != nullptr) {
-                load_run<io_t>(p.z, sp.row, c, t, steps, nc, 234, y);
+                open_run(raw_z, y);
 #pragma unroll
                 for (int k = 0; k < kRun; ++k) {
                     const float2 z = halves(y[k]), f = halves(gy[k]);
                     gy[k] = make_pair(f.x * (z.x * logistic(z.x)), f.y * (z.y * logistic(z.y)));
                 }
             }
-            load_run<io_t>(p.x, sp.row, c, t, steps, nc, 235, u);
-            load_run<io_t>(p.dt, sp.row, c, t, steps, nc, 236, dt);
+            open_run(raw_x, u);
+            open_run(raw_dt, dt);
             make_steps(dt, bias, p.softplus, steps);
 #pragma unroll
             for (int k = 0; k < kRun; ++k) {
@@ -409,12 +564,15 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                 through[k] = 0;
                 bydecay[k] = 0;
             }
-            for (int n0 = 0; n0 < S; n0 += p.slab) {
-                const int count = S - n0 < p.slab ? S - n0 : p.slab;
+            for (int n0 = 0; n0 < S; n0 += slab) {
+                const int count = S - n0 < slab ? S - n0 : slab;
+                Pieces next_B, next_C;
+                next_B.fetch(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
+                next_C.fetch(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
                 __syncthreads();
-                if (S > p.slab) stage_decays<H::CB>(p, c0, c_end, n0, count, decay);
-                stage_projection<io_t, H::TILE>(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
-                stage_projection<io_t, H::TILE>(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
+                if (S > slab) stage_decays<H::CB>(p, c0, c_end, n0, count, decay);
+                next_B.put(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
+                next_C.put(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
                 for (int i = threadIdx.x; i < count * H::CB; i += blockDim.x) {
                     const int n = i / H::CB, cc = i % H::CB;
                     const int64_t at = ((slot0 + i_tile) * S + n0 + n) * p.channels + c0 + cc;

@@ -77,8 +77,16 @@ ssb::View3 view3(const ssb_view_t &v, int dtype, int64_t n, int64_t c, int64_t t
     else if (v.stride[2] == 1 && from_zero && v.stride[1] % 8 == 0 && v.stride[0] % 8 == 0 && aligned(v.data, 16)) r.access = ssb::kRuns;
     return r;
 }
-ssb::ProjView proj_view(const ssb_view_t &v, int64_t n, int64_t g, int64_t s, int64_t t) {
-    return {v.data, v.stride[0], v.stride[1], v.stride[2], v.stride[3], v.data != nullptr ? extent_of(v, {n, g, s, t}) : 0};
+// B or C, and whether 16-byte pieces of it lie whole and aligned: along the states, or along the steps
+// (tiles start at multiples of 32 steps only where sequences start at step 0).
+ssb::ProjView proj_view(const ssb_view_t &v, int dtype, int64_t n, int64_t g, int64_t s, int64_t t, bool from_zero) {
+    const int64_t per = 16 / (int64_t)size_of(dtype);
+    ssb::ProjView r{v.data, v.stride[0], v.stride[1], v.stride[2], v.stride[3], v.data != nullptr ? extent_of(v, {n, g, s, t}) : 0,
+                    ssb::kProjAny};
+    const bool outer = aligned(v.data, 16) && v.stride[0] % per == 0 && v.stride[1] % per == 0;
+    if (outer && v.stride[2] == 1 && v.stride[3] % per == 0 && s % per == 0) r.access = ssb::kProjStates;
+    else if (outer && from_zero && v.stride[3] == 1 && v.stride[2] % per == 0 && t % per == 0) r.access = ssb::kProjSteps;
+    return r;
 }
 ssb::View2 view2(const ssb_view_t &v, int64_t a, int64_t b, int64_t c = 1) {
     return {v.data, v.stride[0], v.stride[1], v.stride[2], v.data != nullptr ? extent_of(v, {a, b, c}) : 0};
@@ -92,7 +100,9 @@ int allow_smem(K kernel, size_t bytes) {
 }
 
 // ---- selective scan -----------------------------------------------------------------------------
-constexpr int kFwdWarps = 4, kBwdWarps = 8;
+// Warps of a CTA: they share the staged B and C, whose staging costs as much as the steps of a tile.
+constexpr int fwd_warps(int tl) { return tl >= 16 ? 8 : 4; }
+constexpr int kBwdWarps = 8;
 
 // Calls f with the split of a warp between time and channels as a compile-time constant.
 template <typename F>
@@ -105,27 +115,24 @@ auto with_split(int tl, F &&f) {
     }
 }
 
-int slab_of(int64_t states) { return (int)std::min<int64_t>(states, ssb::kSlab); }
-
 int64_t channel_blocks(int64_t per_group, int tl, int warps) {
     const int64_t cb = (int64_t)warps * 2 * (32 / tl);
     return (per_group + cb - 1) / cb;
 }
 
-size_t smem_of(bool backward, int tl, int64_t states) {
+size_t smem_of(bool backward, int tl, int64_t states) {  // the largest of any type
     return with_split(tl, [&](auto k) {
         constexpr int TL = decltype(k)::value;
-        return backward ? ssb::selective_bwd_smem<TL, kBwdWarps>(states, slab_of(states))
-                        : ssb::selective_fwd_smem<TL, kFwdWarps>(states, slab_of(states));
+        return backward ? std::max(ssb::selective_bwd_smem<float, TL, kBwdWarps>(states), ssb::selective_bwd_smem<__half, TL, kBwdWarps>(states))
+                        : std::max(ssb::selective_fwd_smem<float, TL, fwd_warps(TL)>(states), ssb::selective_fwd_smem<__half, TL, fwd_warps(TL)>(states));
     });
 }
 
 // Lanes across time: the fewest (they cost shuffles) that give every SM the warps it can hold.
 int split_of(bool backward, int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
-    const int warps = backward ? kBwdWarps : kFwdWarps;
-    const int64_t want = (int64_t)sm_count() * (backward ? 1 : 3);
     for (int tl = 4; tl < 32; tl *= 2)
-        if (groups * channel_blocks(per_group, tl, warps) * std::max<int64_t>(sequences, 1) >= want &&
+        if (groups * channel_blocks(per_group, tl, backward ? kBwdWarps : fwd_warps(tl)) * std::max<int64_t>(sequences, 1) *
+                    (backward ? 1 : fwd_warps(tl)) >= (int64_t)sm_count() * (backward ? 1 : 12) &&
             smem_of(backward, tl, states) <= kSmemLimit)
             return tl;
     return 32;
@@ -171,14 +178,13 @@ ssb::SelectiveArgs selective_args(const ssb_selective_t *p, int tl, int warps) {
     a.states = p->states;
     a.blocks_per_group = (int)channel_blocks(a.per_group, tl, warps);
     a.softplus = p->softplus;
-    a.slab = slab_of(p->states);
     a.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
     a.x = view3(p->x, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
     a.dt = view3(p->dt, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
     a.z = view3(p->z, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
     a.out = view3(p->out, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
-    a.B = proj_view(p->B, p->batch, p->groups, p->states, p->steps);
-    a.C = proj_view(p->C, p->batch, p->groups, p->states, p->steps);
+    a.B = proj_view(p->B, p->dtype, p->batch, p->groups, p->states, p->steps, from_zero);
+    a.C = proj_view(p->C, p->dtype, p->batch, p->groups, p->states, p->steps, from_zero);
     a.A = p->A;
     a.D = p->D;
     a.dt_bias = p->dt_bias;
@@ -331,12 +337,13 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
         using io_t = std::remove_pointer_t<decltype(type)>;
         return with_split(tl, [&](auto k) {
             constexpr int TL = decltype(k)::value;
-            const ssb::SelectiveArgs a = selective_args(p, TL, kFwdWarps);
-            auto kernel = ssb::selective_fwd_kernel<io_t, TL, kFwdWarps>;
-            const size_t smem = ssb::selective_fwd_smem<TL, kFwdWarps>(p->states, a.slab);
+            constexpr int W = fwd_warps(TL);
+            const ssb::SelectiveArgs a = selective_args(p, TL, W);
+            auto kernel = ssb::selective_fwd_kernel<io_t, TL, W>;
+            const size_t smem = ssb::selective_fwd_smem<io_t, TL, W>(p->states);
             if (int rc = allow_smem(kernel, smem)) return rc;
             const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)std::min<int64_t>(count, 65535));
-            kernel<<<grid, kFwdWarps * 32, smem, (cudaStream_t)stream>>>(a);
+            kernel<<<grid, W * 32, smem, (cudaStream_t)stream>>>(a);
             return check_launch("selective_fwd_kernel");
         });
     });
@@ -385,7 +392,7 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
             constexpr int TL = decltype(k)::value;
             const ssb::SelectiveArgs a = selective_args(p, TL, kBwdWarps);
             auto kernel = ssb::selective_bwd_kernel<io_t, TL, kBwdWarps>;
-            const size_t smem = ssb::selective_bwd_smem<TL, kBwdWarps>(p->states, a.slab);
+            const size_t smem = ssb::selective_bwd_smem<io_t, TL, kBwdWarps>(p->states);
             if (int bad = allow_smem(kernel, smem)) return bad;
             const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)parts.parts_seq);
             kernel<<<grid, kBwdWarps * 32, smem, (cudaStream_t)stream>>>(a, q);
@@ -406,8 +413,8 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
     r.part_A = q.part_A;
     r.part_D = q.part_D;
     r.part_bias = q.part_bias;
-    r.gB = proj_view(g->gB, p->batch, p->groups, p->states, p->steps);
-    r.gC = proj_view(g->gC, p->batch, p->groups, p->states, p->steps);
+    r.gB = proj_view(g->gB, p->dtype, p->batch, p->groups, p->states, p->steps, false);
+    r.gC = proj_view(g->gC, p->dtype, p->batch, p->groups, p->states, p->steps, false);
     r.gA = g->gA;
     r.gD = g->gD;
     r.gbias = g->gdt_bias;
