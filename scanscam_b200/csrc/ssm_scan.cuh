@@ -28,7 +28,7 @@ struct ProjView {  // B or C: [N, G, S, T]
 
 struct SelectiveArgs {
     int64_t channels, per_group, groups, states;
-    int blocks_per_group, softplus, tile_log2;  // tile_log2: steps between checkpoints
+    int blocks_per_group, softplus, tile_log2, vec;  // tile_log2: steps between checkpoints; vec: 4 states at a time are whole and aligned
     Sequences seq;
     View3 x, dt, z, out;
     ProjView B, C;
@@ -228,14 +228,9 @@ __device__ __forceinline__ void store_states(float *dst, int64_t seq, const Sele
 __device__ __forceinline__ void make_steps(pair_t (&dt)[kRun], float2 bias, int softplus_on, int steps) {
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
-        float2 f = halves(dt[k]);
-        f.x += bias.x;
-        f.y += bias.y;
-        if (softplus_on) {
-            f.x = softplus(f.x);
-            f.y = softplus(f.y);
-        }
-        dt[k] = k < steps ? make_pair(f.x, f.y) : 0;
+        dt[k] = add2(dt[k], make_pair(bias.x, bias.y));
+        if (softplus_on) dt[k] = softplus2(dt[k]);
+        if (k >= steps) dt[k] = 0;
     }
 }
 
@@ -279,200 +274,6 @@ struct ScanShape {
     static constexpr int TILE = TL * kRun;   // steps of a tile
     static constexpr int PAD = scan_pad(TILE);
 };
-
-#ifndef KATONCE
-#define KATONCE 2
-#endif
-constexpr int kAtOnce = KATONCE;
-// Rounds a number of states up to whole pairs: two states are worked on at a time.
-__host__ __device__ constexpr int64_t even_states(int64_t states) { return (states + 1) & ~(int64_t)1; }
-
-template <typename io_t, int TL, int W>
-__host__ __device__ constexpr size_t selective_fwd_smem(int64_t states) {
-    using H = ScanShape<TL, W>;
-    constexpr int slab = slab_states<io_t, H::TILE, W * 32>();
-    const int64_t even = even_states(states), rows = even < slab ? even : slab;
-    return sizeof(float) * (size_t)(2 * even * H::CB + 2 * rows * H::PAD);
-}
-
-// One tile's states [0, count) of the slab, two at a time: their chains are independent, and hide
-// each other's latency.  `decay` and `carry` start at the slab's first state.
-template <int TL, int W>
-__device__ __forceinline__ void scan_states(const float *decay, float *carry, const float *Bs, const float *Cs, int count, int tl, int cl,
-                                            const pair_t (&dt)[kRun], const pair_t (&u)[kRun], pair_t (&y)[kRun]) {
-    using H = ScanShape<TL, W>;
-#pragma unroll 1
-    for (int n = 0; n < count; n += kAtOnce) {
-        pair_t a[kAtOnce][kRun], b[kAtOnce][kRun], P[kAtOnce], F[kAtOnce], h[kAtOnce], h_in[kAtOnce];
-#pragma unroll
-        for (int q = 0; q < kAtOnce; ++q) {
-            const pair_t A = *reinterpret_cast<const pair_t *>(decay + (n + q) * H::CB + cl);
-            h_in[q] = *reinterpret_cast<const pair_t *>(carry + (n + q) * H::CB + cl);
-            float v[kRun];
-            load8(Bs + (n + q) * H::PAD + tl * kRun, v);
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                a[q][k] = exp2_pair(mul2(dt[k], A));
-                b[q][k] = mul2(u[k], both(v[k]));
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < kAtOnce; ++q) {
-            P[q] = a[q][0];
-            F[q] = b[q][0];
-        }
-#pragma unroll
-        for (int k = 1; k < kRun; ++k) {
-#pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) {
-                F[q] = fma2(a[q][k], F[q], b[q][k]);
-                P[q] = mul2(P[q], a[q][k]);
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < TL; d <<= 1) {
-#pragma unroll
-            for (int q = 0; q < kAtOnce; ++q) {
-                const pair_t P0 = shfl_up2(P[q], d * H::DL), F0 = shfl_up2(F[q], d * H::DL);
-                if (tl >= d) {
-                    F[q] = fma2(P[q], F0, F[q]);
-                    P[q] = mul2(P[q], P0);
-                }
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < kAtOnce; ++q) {
-            const pair_t h_end = fma2(P[q], h_in[q], F[q]);  // the state behind this lane's steps
-            h[q] = shfl_up2(h_end, H::DL);
-            if (tl == 0) h[q] = h_in[q];
-            __syncwarp();  // all lanes have read what is replaced
-            if (tl == TL - 1) *reinterpret_cast<pair_t *>(carry + (n + q) * H::CB + cl) = h_end;
-        }
-#pragma unroll
-        for (int q = 0; q < kAtOnce; ++q) {
-            float v[kRun];
-            load8(Cs + (n + q) * H::PAD + tl * kRun, v);
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                h[q] = fma2(a[q][k], h[q], b[q][k]);
-                y[k] = fma2(h[q], both(v[k]), y[k]);
-            }
-        }
-    }
-}
-
-#ifndef FWD_MINB
-#define FWD_MINB 2
-#endif
-template <typename io_t, int TL, int W>
-__global__ void __launch_bounds__(W * 32, (W == 4 ? FWD_MINB : (FWD_MINB + 1) / 2)) selective_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
-    using H = ScanShape<TL, W>;
-    using Pieces = ProjPieces<io_t, H::TILE, W * 32>;
-    extern __shared__ __align__(16) float smem[];
-    const int S = (int)p.states, even = (int)even_states(S);
-    const int slab = even < Pieces::kSlabStates ? even : Pieces::kSlabStates;  // even: an odd last state has a partner of zeros
-    float *carry = smem;                     // [even][CB]: the state entering the tile
-    float *decay = carry + even * H::CB;     // [even][CB]
-    float *Bs = decay + even * H::CB, *Cs = Bs + slab * H::PAD;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tl = lane / H::DL, cl = warp * H::CW + 2 * (lane % H::DL);
-    const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
-    const int64_t c0 = g * p.per_group + j * H::CB;
-    const int64_t c_end = c0 + H::CB < (g + 1) * p.per_group ? c0 + H::CB : (g + 1) * p.per_group;
-    const int64_t c = c0 + cl;
-    const int nc = c_end - c >= 2 ? 2 : (c_end > c ? 1 : 0);  // channels of this thread that exist
-    float2 D = make_float2(0.0f, 0.0f), bias = D;
-    if (p.D != nullptr) {
-        if (nc > 0) D.x = load_one(p.D, c, p.channels, 212);
-        if (nc > 1) D.y = load_one(p.D, c + 1, p.channels, 212);
-    }
-    if (p.dt_bias != nullptr) {
-        if (nc > 0) bias.x = load_one(p.dt_bias, c, p.channels, 213);
-        if (nc > 1) bias.y = load_one(p.dt_bias, c + 1, p.channels, 213);
-    }
-    stage_decays<H::CB>(p, c0, c_end, 0, S, decay);
-    if (even != S)  // the partner of an odd last state: decay 1, no input, no read-out
-        for (int i = threadIdx.x; i < H::CB; i += W * 32) decay[S * H::CB + i] = 0.0f;
-
-    for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
-        const Span sp = span_of(p.seq, s);
-        load_states<H::CB, H::CW>(p.state, s, p, c0, c_end, warp, lane, 214, carry);
-        if (even != S && tl == 0) *reinterpret_cast<pair_t *>(carry + S * H::CB + cl) = 0;
-        const int64_t slot0 = p.checkpoints != nullptr ? checkpoint_base(p, s, sp.start) : 0;
-        RawRun<io_t> raw_x, raw_dt;
-        Pieces next_B, next_C;
-        const auto fetch = [&](int64_t t0) {  // this thread's runs of the tile at t0
-            const int64_t left = sp.length - t0 - tl * kRun;
-            const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
-            fetch_run(p.x, sp.row, c, sp.start + t0 + tl * kRun, steps, nc, 215, raw_x);
-            fetch_run(p.dt, sp.row, c, sp.start + t0 + tl * kRun, steps, nc, 216, raw_dt);
-        };
-        const auto fetch_projections = [&](int64_t t0, int n0) {
-            const int count = S - n0 < slab ? S - n0 : slab;
-            next_B.fetch(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
-            next_C.fetch(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0);
-        };
-        if (sp.length > 0) {
-            fetch(0);
-            fetch_projections(0, 0);
-        }
-        for (int64_t t0 = 0; t0 < sp.length; t0 += H::TILE) {
-            const int64_t left = sp.length - t0 - tl * kRun;
-            const int steps = left >= kRun ? kRun : (left > 0 ? (int)left : 0);
-            const int64_t t = sp.start + t0 + tl * kRun;
-            pair_t dt[kRun], u[kRun], y[kRun];
-            open_run(raw_x, u);
-            open_run(raw_dt, dt);
-            make_steps(dt, bias, p.softplus, steps);
-            const pair_t Dp = make_pair(D.x, D.y);
-#pragma unroll
-            for (int k = 0; k < kRun; ++k) {
-                y[k] = mul2(Dp, u[k]);
-                u[k] = mul2(dt[k], u[k]);  // from here on dt * x
-            }
-            if (p.checkpoints != nullptr && (t0 & ((1ll << p.tile_log2) - 1)) == 0) {
-                const int64_t slot = slot0 + (t0 >> p.tile_log2);
-                for (int n = tl; n < S; n += TL) {
-                    const int64_t at = (slot * S + n) * p.channels + c;
-                    const float *from = carry + n * H::CB + cl;
-                    if (nc > 0) store_one(p.checkpoints, at, p.checkpoint_slots * S * p.channels, 217, from[0]);
-                    if (nc > 1) store_one(p.checkpoints, at + 1, p.checkpoint_slots * S * p.channels, 217, from[1]);
-                }
-                __syncwarp();
-            }
-            for (int n0 = 0; n0 < S; n0 += slab) {
-                const int count = S - n0 < slab ? S - n0 : slab;
-                __syncthreads();
-                next_B.put(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
-                next_C.put(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
-                if (count & 1)
-                    for (int i = threadIdx.x; i < H::PAD; i += W * 32) Bs[count * H::PAD + i] = Cs[count * H::PAD + i] = 0.0f;
-                __syncthreads();
-                // what the next slab needs is under way while this one is worked on
-                if (n0 + slab < S) {
-                    fetch_projections(t0, n0 + slab);
-                } else if (t0 + H::TILE < sp.length) {
-                    fetch(t0 + H::TILE);
-                    fetch_projections(t0 + H::TILE, 0);
-                }
-                scan_states<TL, W>(decay + n0 * H::CB, carry + n0 * H::CB, Bs, Cs, count, tl, cl, dt, u, y);
-            }
-            __syncwarp();
-            if (p.z.data != nullptr) {
-                load_run<io_t>(p.z, sp.row, c, t, steps, nc, 218, u);
-#pragma unroll
-                for (int k = 0; k < kRun; ++k) {
-                    const float2 z = halves(u[k]), f = halves(y[k]);
-                    y[k] = make_pair(f.x * (z.x * logistic(z.x)), f.y * (z.y * logistic(z.y)));
-                }
-            }
-            store_run<io_t>(p.out, sp.row, c, t, steps, nc, 219, y);
-        }
-        if (p.state_out != nullptr) store_states<H::CB, H::CW>(p.state_out, s, p, c0, c_end, warp, lane, 220, carry);
-        zero_uncovered<io_t>(p.seq, s, sp, p.out, c0, c_end, 219);
-        __syncthreads();  // the staged tile of this sequence is no longer read
-    }
-}
 
 // ---- backward -----------------------------------------------------------------------------------
 // Tiles run from the last to the first.  Each starts from its checkpoint (the state the forward
@@ -574,9 +375,9 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                 next_B.put(p.B, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Bs);
                 next_C.put(p.C, sp.row, g, n0, count, sp.start + t0, sp.length - t0, Cs);
                 for (int i = threadIdx.x; i < count * H::CB; i += blockDim.x) {
-                    const int n = i / H::CB, cc = i % H::CB;
-                    const int64_t at = ((slot0 + i_tile) * S + n0 + n) * p.channels + c0 + cc;
-                    first[i] = c0 + cc < c_end ? load_one(p.checkpoints, at, p.checkpoint_slots * S * p.channels, 237) : 0.0f;
+                    const int cc = i / count, n = i - cc * count;
+                    const int64_t at = ((slot0 + i_tile) * p.channels + c0 + cc) * S + n0 + n;
+                    first[n * H::CB + cc] = c0 + cc < c_end ? load_one(p.checkpoints, at, p.checkpoint_slots * S * p.channels, 237) : 0.0f;
                 }
                 for (int i = threadIdx.x; i < count * H::PAD; i += blockDim.x) {
                     sumB[i] = 0.0f;

@@ -9,6 +9,7 @@
 
 #include "host_common.h"
 #include "short_conv.cuh"
+#include "ssm_forward.cuh"
 #include "ssm_scan.cuh"
 #include "ssm_step.cuh"
 
@@ -100,9 +101,19 @@ int allow_smem(K kernel, size_t bytes) {
 }
 
 // ---- selective scan -----------------------------------------------------------------------------
-// Warps of a CTA: they share the staged B and C, whose staging costs as much as the steps of a tile.
-constexpr int fwd_warps(int tl) { return tl >= 16 ? 8 : 4; }
 constexpr int kBwdWarps = 8;
+
+// Calls f with the lanes that share a channel and the states each of them holds.
+template <typename F>
+auto with_lanes(int64_t states, F &&f) {
+    using std::integral_constant;
+    if (states <= 8) return f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
+    if (states <= 16) return f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
+    if (states <= 32) return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
+    if (states <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    if (states <= 128) return f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+    return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+}
 
 // Calls f with the split of a warp between time and channels as a compile-time constant.
 template <typename F>
@@ -120,20 +131,18 @@ int64_t channel_blocks(int64_t per_group, int tl, int warps) {
     return (per_group + cb - 1) / cb;
 }
 
-size_t smem_of(bool backward, int tl, int64_t states) {  // the largest of any type
+size_t smem_of(int tl, int64_t states) {  // the largest of any type
     return with_split(tl, [&](auto k) {
         constexpr int TL = decltype(k)::value;
-        return backward ? std::max(ssb::selective_bwd_smem<float, TL, kBwdWarps>(states), ssb::selective_bwd_smem<__half, TL, kBwdWarps>(states))
-                        : std::max(ssb::selective_fwd_smem<float, TL, fwd_warps(TL)>(states), ssb::selective_fwd_smem<__half, TL, fwd_warps(TL)>(states));
+        return std::max(ssb::selective_bwd_smem<float, TL, kBwdWarps>(states), ssb::selective_bwd_smem<__half, TL, kBwdWarps>(states));
     });
 }
 
-// Lanes across time: the fewest (they cost shuffles) that give every SM the warps it can hold.
-int split_of(bool backward, int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
+// Lanes across time: the fewest (they cost shuffles) that give every SM a CTA.
+int split_of(int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
     for (int tl = 4; tl < 32; tl *= 2)
-        if (groups * channel_blocks(per_group, tl, backward ? kBwdWarps : fwd_warps(tl)) * std::max<int64_t>(sequences, 1) *
-                    (backward ? 1 : fwd_warps(tl)) >= (int64_t)sm_count() * (backward ? 1 : 12) &&
-            smem_of(backward, tl, states) <= kSmemLimit)
+        if (groups * channel_blocks(per_group, tl, kBwdWarps) * std::max<int64_t>(sequences, 1) >= (int64_t)sm_count() &&
+            smem_of(tl, states) <= kSmemLimit)
             return tl;
     return 32;
 }
@@ -162,21 +171,37 @@ int check_selective(const ssb_selective_t *p, bool data) {
 int64_t count_of(const ssb_selective_t *p) { return p->offsets != nullptr ? p->sequences : p->batch; }
 
 int backward_split(const ssb_selective_t *p) {
-    return split_of(true, p->channels / p->groups, p->groups, count_of(p), p->states);
+    return split_of(p->channels / p->groups, p->groups, count_of(p), p->states);
 }
 int64_t checkpoint_slots(const ssb_selective_t *p) {
     const int64_t tile = backward_split(p) * ssb::kRun;
     return p->offsets != nullptr ? p->steps / tile + p->sequences + 1 : p->batch * ((p->steps + tile - 1) / tile);
 }
 
-ssb::SelectiveArgs selective_args(const ssb_selective_t *p, int tl, int warps) {
+// How pieces of all the forward's [N, C, T] operands may be fetched: the same way for each of them.
+int tile_access(const ssb_selective_t *p) {
+    const int64_t per = 16 / (int64_t)size_of(p->dtype);
+    bool channels = p->groups == 1 || p->channels / p->groups % per == 0;  // blocks of channels start at whole pieces
+    bool steps = p->offsets == nullptr && p->steps % per == 0;
+    for (const ssb_view_t *v : {&p->x, &p->dt, &p->z, &p->out}) {
+        if (v->data == nullptr) continue;
+        const bool base = aligned(v->data, 16) && v->stride[0] % per == 0;
+        channels = channels && base && v->stride[1] == 1 && v->stride[2] % per == 0;
+        steps = steps && base && v->stride[2] == 1 && v->stride[1] % per == 0;
+    }
+    return channels ? ssb::kTileChannels : (steps ? ssb::kTileSteps : ssb::kTileAny);
+}
+
+ssb::SelectiveArgs selective_args(const ssb_selective_t *p, int64_t blocks_per_group) {
     ssb::SelectiveArgs a{};
     const bool from_zero = p->offsets == nullptr, even = p->groups == 1 || p->channels / p->groups % 2 == 0;
     a.channels = p->channels;
     a.groups = p->groups;
     a.per_group = p->channels / p->groups;
     a.states = p->states;
-    a.blocks_per_group = (int)channel_blocks(a.per_group, tl, warps);
+    a.blocks_per_group = (int)blocks_per_group;
+    a.vec = p->states % 4 == 0;
+    for (const void *f : {(const void *)p->A, (const void *)p->state, (const void *)p->state_out, (const void *)p->checkpoints}) a.vec = a.vec && aligned(f, 16);
     a.softplus = p->softplus;
     a.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
     a.x = view3(p->x, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
@@ -331,20 +356,21 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
     if (p->channels == 0 || count == 0) return SSB_OK;
     if (p->steps > 0 && p->batch > 0)
         if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
-    int tl = split_of(false, p->channels / p->groups, p->groups, count, p->states);
-    if (p->checkpoints != nullptr) tl = std::min(tl, backward_split(p));  // checkpoints lie at tile starts
     return with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
-        return with_split(tl, [&](auto k) {
-            constexpr int TL = decltype(k)::value;
-            constexpr int W = fwd_warps(TL);
-            const ssb::SelectiveArgs a = selective_args(p, TL, W);
-            auto kernel = ssb::selective_fwd_kernel<io_t, TL, W>;
-            const size_t smem = ssb::selective_fwd_smem<io_t, TL, W>(p->states);
+        return with_lanes(p->states, [&](auto lanes, auto each) {
+            constexpr int LN = decltype(lanes)::value, SPL = decltype(each)::value;
+            using H = ssb::LaneShape<LN, SPL>;
+            const int64_t per_group = p->channels / p->groups;
+            ssb::SelectiveArgs a = selective_args(p, (per_group + H::CB - 1) / H::CB);
+            a.x.access = a.dt.access = a.z.access = a.out.access = tile_access(p);
+            if (a.B.access != a.C.access) a.B.access = a.C.access = ssb::kProjAny;
+            auto kernel = ssb::selective_lane_fwd_kernel<io_t, LN, SPL>;
+            constexpr size_t smem = ssb::selective_lane_smem<LN, SPL>();
             if (int rc = allow_smem(kernel, smem)) return rc;
             const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)std::min<int64_t>(count, 65535));
-            kernel<<<grid, W * 32, smem, (cudaStream_t)stream>>>(a);
-            return check_launch("selective_fwd_kernel");
+            kernel<<<grid, H::THREADS, smem, (cudaStream_t)stream>>>(a);
+            return check_launch("selective_lane_fwd_kernel");
         });
     });
 }
@@ -390,7 +416,7 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
         using io_t = std::remove_pointer_t<decltype(type)>;
         return with_split(backward_split(p), [&](auto k) {
             constexpr int TL = decltype(k)::value;
-            const ssb::SelectiveArgs a = selective_args(p, TL, kBwdWarps);
+            const ssb::SelectiveArgs a = selective_args(p, channel_blocks(p->channels / p->groups, TL, kBwdWarps));
             auto kernel = ssb::selective_bwd_kernel<io_t, TL, kBwdWarps>;
             const size_t smem = ssb::selective_bwd_smem<io_t, TL, kBwdWarps>(p->states);
             if (int bad = allow_smem(kernel, smem)) return bad;
