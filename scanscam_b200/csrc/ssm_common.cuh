@@ -84,47 +84,42 @@ __device__ __forceinline__ float exp_accurate(float x) {
     const float e = exp2_approx(hi);
     return isfinite(hi) ? fmaf(e, lo * kLn2, e) : e;
 }
-// 1 / (1 + e^-x).  The plain form is off by up to |x| 2^-24 of the value where x is far below zero,
-// which a gate x * logistic(x) does not feel; the derivative of softplus does (its arguments are
-// around -5), and takes the other.
-__device__ __forceinline__ float logistic(float x) { return __fdividef(1.0f, 1.0f + exp2_approx(-x * kLog2e)); }
-__device__ __forceinline__ float logistic_accurate(float x) { return __fdividef(1.0f, 1.0f + exp_accurate(-x)); }
-
-__device__ __forceinline__ float reciprocal_approx(float x) {  // x in [2, 3]: no range to look after
+__device__ __forceinline__ float reciprocal_approx(float x) {  // 0 for infinity; one unit in the last place
     float y;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// 1 / (1 + e^-x).  The plain form is off by up to |x| 2^-24 of the value where x is far below zero,
+// which a gate x * logistic(x) does not feel; the derivative of softplus does (its arguments are
+// around -5), and takes the other.
+__device__ __forceinline__ float logistic(float x) { return reciprocal_approx(1.0f + exp2_approx(-x * kLog2e)); }
+__device__ __forceinline__ float logistic_accurate(float x) { return __fdividef(1.0f, 1.0f + exp_accurate(-x)); }
+
 __device__ __forceinline__ float relu_or_nan(float v) {
     float y;
     asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(v));
     return y;
 }
-// log(1 + e^v) = max(v, 0) + log1p(e^-|v|), for two values.  log1p(e) = 2 atanh(e / (2 + e)); the quotient is at
-// most 1/3, so the odd series up to the 15th power leaves 2e-9 of the value.  Below -87 the result stays at
-// e^-87 = 1.6e-38, where the type's normal range ends.  The exponential as in exp_accurate.
+// log(1 + e^v) = max(v, 0) + log1p(e^-|v|).  log1p(e) = 2 atanh(s) with s = e / (2 + e) of at most 1/3;
+// atanh(s) = s + s q P(q), q = s^2, where P is a cubic fitted (Chebyshev, weighted with q) to
+// (atanh(s) / s - 1) / q on [0, 1/9]: 4.6e-9 of the value.  Below -87 the result stays at e^-87 = 1.6e-38,
+// where the type's normal range ends.  The exponential as in exp_accurate.
+__device__ __forceinline__ float softplus(float v) {
+    const float x = fmaxf(-fabsf(v), -87.0f);
+    const float hi = x * kLog2e;
+    const float lo = fmaf(x, 1.925963033500945e-8f, fmaf(x, kLog2e, -hi));
+    float e = exp2_approx(hi);
+    e = fmaf(e, lo * kLn2, e);
+    const float s = e * reciprocal_approx(e + 2.0f), q = s * s;
+    float p = fmaf(q, 0.13988047f, 0.14004979f);
+    p = fmaf(p, q, 0.20010476f);
+    p = fmaf(p, q, 0.33333215f);
+    return fmaf(fmaf(p * q, s, s), 2.0f, relu_or_nan(v));
+}
 __device__ __forceinline__ pair_t softplus2(pair_t v) {
     const float2 f = halves(v);
-    const pair_t x = make_pair(fmaxf(-fabsf(f.x), -87.0f), fmaxf(-fabsf(f.y), -87.0f));
-    const pair_t hi = mul2(x, both(kLog2e));
-    const float2 h = halves(hi);
-    pair_t lo = fma2(x, both(kLog2e), make_pair(-h.x, -h.y));
-    lo = fma2(x, both(1.925963033500945e-8f), lo);
-    pair_t e = exp2_pair(hi);
-    e = fma2(e, mul2(lo, both(kLn2)), e);
-    const float2 d = halves(add2(e, both(2.0f)));
-    const pair_t s = mul2(e, make_pair(reciprocal_approx(d.x), reciprocal_approx(d.y)));
-    const pair_t q = mul2(s, s);
-    pair_t p = fma2(q, both(1.0f / 15), both(1.0f / 13));
-    p = fma2(p, q, both(1.0f / 11));
-    p = fma2(p, q, both(1.0f / 9));
-    p = fma2(p, q, both(1.0f / 7));
-    p = fma2(p, q, both(1.0f / 5));
-    p = fma2(p, q, both(1.0f / 3));
-    p = fma2(mul2(p, q), s, s);
-    return fma2(p, both(2.0f), make_pair(relu_or_nan(f.x), relu_or_nan(f.y)));
+    return make_pair(softplus(f.x), softplus(f.y));
 }
-__device__ __forceinline__ float softplus(float v) { return halves(softplus2(both(v))).x; }
 
 // ---- views ------------------------------------------------------------------------------------
 // How runs of 8 steps x 2 channels of a [N, C, T] view may be fetched:

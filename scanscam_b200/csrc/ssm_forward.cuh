@@ -8,8 +8,8 @@
 // LN lanes share a channel, each with SPL of its states (4; 8 beyond 128 states); a warp holds
 // 32 / LN channels and walks the steps in order.  Per step and 4 states a lane issues 4 exponentials,
 // 8 packed operations (exponent, input, recurrence, read-out, two states each) and 3 shared loads.
-// The read-out is summed over the LN lanes once per LN steps, in LN - 1 shuffles that leave each lane
-// with the sum of one step.  A tile of 32 steps is put into shared memory by the whole CTA: (dt, x)
+// The read-out is summed over the LN lanes for groups of steps, so that each lane is left with the sum
+// of one step (LN = 4: 3 shuffles for 4 steps).  A tile of 32 steps is put into shared memory by the whole CTA: (dt, x)
 // after the softplus, B and C as fp32; the next tile's bytes are fetched meanwhile.  The sums take the
 // place of the steps in shared memory and leave, gated, with 16-byte stores.
 #pragma once
@@ -23,78 +23,77 @@ constexpr int kTile = 32;  // steps of a tile
 // 16-byte pieces of a tile of a [N, C, T] view: 8 (4) adjacent channels of a step, or adjacent steps of a channel.
 enum TileAccess : int { kTileAny = 0, kTileChannels = 1, kTileSteps = 2 };
 
+// Which pieces of a tile a thread handles: always the same channels, steps `next` apart.
 template <typename io_t, int CB, int THREADS>
-struct TilePieces {
+struct TileShare {
     static constexpr int kPer = 16 / (int)sizeof(io_t);
     static constexpr int kPieces = (kTile * CB / kPer + THREADS - 1) / THREADS;
-    static_assert(CB % kPer == 0, "whole pieces of channels");
-    uint4 piece[kPieces];
+    static_assert(CB % kPer == 0 && THREADS % CB == 0, "whole pieces of channels");
+    bool by_step, whole, works;  // whole: one 16-byte access; works: not a thread too many
+    int t, c, next, channels;    // first step, first channel, steps between pieces, channels of the CTA
 
-    // where piece j of this thread lies in the tile: first step and channel
-    __device__ __forceinline__ static bool place(int access, int j, int &t, int &c) {
-        const int i = threadIdx.x + j * THREADS;
-        if (access == kTileSteps) {
-            c = i % CB;
-            t = i / CB * kPer;
-        } else {
-            c = i % (CB / kPer) * kPer;
-            t = i / (CB / kPer);
-        }
-        return i < kTile * CB / kPer;
+    __device__ __forceinline__ TileShare(int access, int tid, int channels_) : channels(channels_) {
+        by_step = access == kTileSteps;
+        c = by_step ? tid % CB : tid % (CB / kPer) * kPer;
+        t = by_step ? tid / CB * kPer : tid / (CB / kPer);
+        next = by_step ? THREADS / CB * kPer : THREADS / (CB / kPer);
+        works = t < kTile && c < channels;
+        whole = access == kTileChannels ? c + kPer <= channels : by_step;
     }
-    __device__ __forceinline__ void fetch(const View3 &v, int64_t row, int64_t c0, int channels, int64_t t0, int64_t steps, int site) {
+    // the address of the thread's first piece in the tile that starts at step t0
+    __device__ __forceinline__ int64_t offset(const View3 &v, int64_t row, int64_t c0, int64_t t0) const {
+        return row * v.sn + (c0 + c) * v.sc + (t0 + t) * v.st;
+    }
+    // pieces of the tile at `at`, zero behind `left` steps; the elements of a piece along the steps that lie behind
+    // are whatever memory holds
+    __device__ __forceinline__ void fetch(const View3 &v, int64_t at, int left, int site, uint4 (&piece)[kPieces]) const {
         const io_t *base = static_cast<const io_t *>(v.data);
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
-            int t, c;
             piece[j] = make_uint4(0, 0, 0, 0);
-            if (!place(v.access, j, t, c) || t >= steps || c >= channels) continue;
-            const int64_t at = row * v.sn + (c0 + c) * v.sc + (t0 + t) * v.st;
-            const bool whole = v.access == kTileChannels ? c + kPer <= channels : v.access == kTileSteps;
-            if (whole) {
-                if (SSB_VECTOR_OK(base + at, 16, at + kPer - 1, v.extent, site)) piece[j] = *reinterpret_cast<const uint4 *>(base + at);
-            } else {
-                io_t e[kPer];
+            if (works && t + j * next < left) {
+                const int64_t i = at + j * next * v.st;
+                if (whole) {
+                    if (SSB_VECTOR_OK(base + i, 16, i + kPer - 1, v.extent, site)) piece[j] = *reinterpret_cast<const uint4 *>(base + i);
+                } else {
+                    io_t e[kPer];
 #pragma unroll
-                for (int k = 0; k < kPer; ++k) {
-                    const int64_t i = at + k * v.sc;
-                    e[k] = io_t(0.0f);
-                    if (c + k < channels && SSB_INDEX_OK(i, v.extent, site)) e[k] = base[i];
+                    for (int k = 0; k < kPer; ++k) {
+                        e[k] = io_t(0.0f);
+                        if (c + k < channels && SSB_INDEX_OK(i + k * v.sc, v.extent, site)) e[k] = base[i + k * v.sc];
+                    }
+                    memcpy(&piece[j], e, 16);
                 }
-                memcpy(&piece[j], e, 16);
             }
         }
     }
-    // element k of piece j as fp32; elements behind the last step are zero
-    __device__ __forceinline__ void open(int j, float (&f)[kPer]) const {
+    __device__ __forceinline__ static void open(const uint4 &piece, float (&f)[kPer]) {
         if constexpr (sizeof(io_t) == 2) {
-            unpack2<io_t>(piece[j].x, f[0], f[1]);
-            unpack2<io_t>(piece[j].y, f[2], f[3]);
-            unpack2<io_t>(piece[j].z, f[4], f[5]);
-            unpack2<io_t>(piece[j].w, f[6], f[7]);
+            unpack2<io_t>(piece.x, f[0], f[1]);
+            unpack2<io_t>(piece.y, f[2], f[3]);
+            unpack2<io_t>(piece.z, f[4], f[5]);
+            unpack2<io_t>(piece.w, f[6], f[7]);
         } else {
-            f[0] = __uint_as_float(piece[j].x); f[1] = __uint_as_float(piece[j].y);
-            f[2] = __uint_as_float(piece[j].z); f[3] = __uint_as_float(piece[j].w);
+            f[0] = __uint_as_float(piece.x); f[1] = __uint_as_float(piece.y);
+            f[2] = __uint_as_float(piece.z); f[3] = __uint_as_float(piece.w);
         }
     }
-    __device__ __forceinline__ static void store(const View3 &v, int64_t row, int64_t c0, int channels, int64_t t0, int64_t steps, int site,
-                                                 int t, int c, const float (&f)[kPer]) {
+    __device__ __forceinline__ void store(const View3 &v, int64_t at, int j, int left, int site, const float (&f)[kPer]) const {
         io_t *base = static_cast<io_t *>(v.data);
-        if (t >= steps || c >= channels) return;
-        const int64_t at = row * v.sn + (c0 + c) * v.sc + (t0 + t) * v.st;
-        const bool whole = v.access == kTileChannels ? c + kPer <= channels : v.access == kTileSteps && t + kPer <= steps;
-        if (whole) {
-            if (!SSB_VECTOR_OK(base + at, 16, at + kPer - 1, v.extent, site)) return;
+        const int64_t i = at + j * next * v.st;
+        const int here = t + j * next;
+        if (!works || here >= left) return;
+        if (whole && (!by_step || here + kPer <= left)) {
+            if (!SSB_VECTOR_OK(base + i, 16, i + kPer - 1, v.extent, site)) return;
             if constexpr (sizeof(io_t) == 2)
-                *reinterpret_cast<uint4 *>(base + at) = make_uint4(pack2<io_t>(f[0], f[1]), pack2<io_t>(f[2], f[3]),
-                                                                   pack2<io_t>(f[4], f[5]), pack2<io_t>(f[6], f[7]));
+                *reinterpret_cast<uint4 *>(base + i) = make_uint4(pack2<io_t>(f[0], f[1]), pack2<io_t>(f[2], f[3]),
+                                                                  pack2<io_t>(f[4], f[5]), pack2<io_t>(f[6], f[7]));
             else
-                *reinterpret_cast<float4 *>(base + at) = make_float4(f[0], f[1], f[2], f[3]);
+                *reinterpret_cast<float4 *>(base + i) = make_float4(f[0], f[1], f[2], f[3]);
         } else {
 #pragma unroll
             for (int k = 0; k < kPer; ++k) {
-                const int dc = v.access == kTileSteps ? 0 : k, dt = v.access == kTileSteps ? k : 0;
-                if (c + dc < channels && t + dt < steps) store_one(base, at + dc * v.sc + dt * v.st, v.extent, site, f[k]);
+                if (by_step ? here + k < left : c + k < channels) store_one(base, i + k * (by_step ? v.st : v.sc), v.extent, site, f[k]);
             }
         }
     }
@@ -108,8 +107,8 @@ struct ProjectionPieces {
     static constexpr int kPieces = (2 * kEach + THREADS - 1) / THREADS;
     uint4 piece[kPieces];
 
-    __device__ __forceinline__ static bool place(int access, int j, int &which, int &t, int &n) {
-        const int i = threadIdx.x + j * THREADS, r = i % kEach;
+    __device__ __forceinline__ static bool place(int access, int tid, int j, int &which, int &t, int &n) {
+        const int i = tid + j * THREADS, r = i % kEach;
         which = i / kEach;
         if (access == kProjSteps) {
             n = r % SP;
@@ -120,12 +119,12 @@ struct ProjectionPieces {
         }
         return i < 2 * kEach;
     }
-    __device__ __forceinline__ void fetch(const ProjView &B, const ProjView &C, int64_t row, int64_t g, int states, int64_t t0, int64_t steps) {
+    __device__ __forceinline__ void fetch(int tid, const ProjView &B, const ProjView &C, int64_t row, int64_t g, int states, int64_t t0, int64_t steps) {
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
             int which, t, n;
             piece[j] = make_uint4(0, 0, 0, 0);
-            if (!place(B.access, j, which, t, n) || t >= steps || n >= states) continue;
+            if (!place(B.access, tid, j, which, t, n) || t >= steps || n >= states) continue;
             const ProjView &v = which ? C : B;
             const io_t *base = static_cast<const io_t *>(v.data);
             const int64_t at = row * v.sn + g * v.sg + n * v.ss + (t0 + t) * v.st;
@@ -143,11 +142,11 @@ struct ProjectionPieces {
         }
     }
     // into [2][step][SP] floats
-    __device__ __forceinline__ void put(int access, int64_t steps, float *smem) const {
+    __device__ __forceinline__ void put(int tid, int access, int64_t steps, float *smem) const {
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
             int which, t, n;
-            if (!place(access, j, which, t, n)) continue;
+            if (!place(access, tid, j, which, t, n)) continue;
             float f[kPer];
             if constexpr (sizeof(io_t) == 2) {
                 unpack2<io_t>(piece[j].x, f[0], f[1]);
@@ -170,11 +169,12 @@ struct ProjectionPieces {
     }
 };
 
-// Sums v[i] of step i over the LN lanes of a channel; lane q of them is left with step q's sum.
-template <int LN>
-__device__ __forceinline__ float sum_and_spread(float (&v)[LN], int q) {
+// Sums v[i] of step i over the LN lanes of a channel; lane q of them is left with the sum of step q mod STEPS.
+template <int LN, int STEPS>
+__device__ __forceinline__ float sum_and_spread(float (&v)[STEPS], int q) {
+    static_assert(STEPS <= LN, "a lane is left with one step");
 #pragma unroll
-    for (int half = LN / 2; half >= 1; half >>= 1) {
+    for (int half = STEPS / 2; half >= 1; half >>= 1) {
         const bool upper = (q & half) != 0;
 #pragma unroll
         for (int i = 0; i < half; ++i) {
@@ -182,6 +182,8 @@ __device__ __forceinline__ float sum_and_spread(float (&v)[LN], int q) {
             v[i] = keep + __shfl_xor_sync(kFullMask, give, half);
         }
     }
+#pragma unroll
+    for (int d = STEPS; d < LN; d <<= 1) v[0] += __shfl_xor_sync(kFullMask, v[0], d);
     return v[0];
 }
 
@@ -189,9 +191,9 @@ template <int LN, int SPL>
 struct LaneShape {
     static constexpr int SP = LN * SPL;                  // states, padded
     static constexpr int DL = 32 / LN;                   // channels of a warp
-    static constexpr int W = LN >= 16 ? 8 : 4;           // warps
+    static constexpr int W = LN >= 16 ? 8 : 4;           // warps that scan, and as many that move tiles
     static constexpr int CB = W * DL;                    // channels of a CTA
-    static constexpr int THREADS = W * 32;
+    static constexpr int THREADS = W * 32;               // of either kind
 };
 
 // Where the pair of step t and channel c lies in a tile of pairs [step][channel].  A thread writes 4 adjacent
@@ -205,7 +207,7 @@ __device__ __forceinline__ int pair_slot(int t, int c) {
 template <int LN, int SPL>
 __host__ __device__ constexpr size_t selective_lane_smem() {
     using H = LaneShape<LN, SPL>;
-    return sizeof(float) * 2 * (size_t)(2 * kTile * H::CB + 2 * kTile * H::SP);  // two tiles of (dt, x) and of B and C
+    return sizeof(float) * (size_t)(3 * 2 * kTile * H::CB + 2 * 2 * kTile * H::SP);  // three tiles of (dt, x), two of B and C
 }
 
 // SPL states of the lane's channel at [..., S] floats, zero behind the last.
@@ -269,148 +271,213 @@ __device__ __forceinline__ void load_lane_projection(const float *smem, pair_t (
     }
 }
 
+// One group of steps in registers: what a lane needs of them.
+template <int STEPS, int SPL>
+struct StepGroup {
+    float2 dx[STEPS];
+    pair_t b[STEPS][SPL / 2], r[STEPS][SPL / 2];
+};
+
 template <typename io_t, int LN, int SPL>
-__global__ void __launch_bounds__(LaneShape<LN, SPL>::THREADS) selective_lane_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
+__global__ void __launch_bounds__(2 * LaneShape<LN, SPL>::THREADS, LaneShape<LN, SPL>::W == 4 ? 2 : 1) selective_lane_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
     using H = LaneShape<LN, SPL>;
-    using Tile = TilePieces<io_t, H::CB, H::THREADS>;
+    using Share = TileShare<io_t, H::CB, H::THREADS>;
     using Proj = ProjectionPieces<io_t, H::SP, H::THREADS>;
-    constexpr int kGroup = LN > 4 ? LN : 4;  // steps worked on together
+    constexpr int kGroup = 8;                      // steps whose sums are exchanged together
+    constexpr int kAhead = SPL > 4 ? 2 : 4;        // steps loaded together, one such part ahead of their use
     extern __shared__ __align__(16) float smem[];
-    float2 *const all_steps = reinterpret_cast<float2 *>(smem);  // [2 tiles][step][channel]: (dt, x), then (y, x)
-    float *const all_proj = smem + 4 * kTile * H::CB;            // [2 tiles][B, C][step][SP]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int q = lane % LN, cl = warp * H::DL + lane / LN;  // lanes of a channel are neighbours
+    float2 *const all_steps = reinterpret_cast<float2 *>(smem);  // [3 tiles][step][channel]: (dt, x), then (y, x)
+    float *const all_proj = smem + 3 * 2 * kTile * H::CB;        // [2 tiles][B, C][step][SP]
+    const bool scans = threadIdx.x < H::THREADS;
+    const int tid = scans ? threadIdx.x : threadIdx.x - H::THREADS;
     const int64_t g = blockIdx.x / p.blocks_per_group, j = blockIdx.x % p.blocks_per_group;
     const int64_t c0 = g * p.per_group + j * H::CB, left_channels = (g + 1) * p.per_group - c0;
     const int channels = left_channels < H::CB ? (int)left_channels : H::CB;
-    const bool live = cl < channels;
-    const int64_t c = c0 + (live ? cl : 0);
-    const int S = (int)p.states, have = live ? (S - q * SPL < SPL ? S - q * SPL : SPL) : 0;  // states of this lane (none: < 1)
-    pair_t A[SPL / 2];
-    load_lane_decays<SPL>(p.A, c * S + q * SPL, have, p.vec, p.channels * S, 261, A);
-    const float D = q == 0 && p.D != nullptr ? load_one(p.D, c, p.channels, 212) : 0.0f;
+    const int S = (int)p.states;
 
-    for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
-        const Span sp = span_of(p.seq, s);
-        const int64_t state_at = (s * p.channels + c) * S + q * SPL, state_extent = p.seq.count * p.channels * S;
-        pair_t h[SPL / 2] = {};
-        if (p.state != nullptr) load_lane_states<SPL>(p.state, state_at, have, p.vec, state_extent, 214, h);
-        const int64_t slot0 = p.checkpoints != nullptr ? checkpoint_base(p, s, sp.start) : 0;
-        Tile next_x, next_dt, next_z;
-        Proj next_proj;
-        const auto fetch = [&](int64_t t0) {
-            next_x.fetch(p.x, sp.row, c0, channels, sp.start + t0, sp.length - t0, 215);
-            next_dt.fetch(p.dt, sp.row, c0, channels, sp.start + t0, sp.length - t0, 216);
-            next_proj.fetch(p.B, p.C, sp.row, g, S, sp.start + t0, sp.length - t0);
-        };
-        if (sp.length > 0) fetch(0);
-        int buffer = 0;
-        for (int64_t t0 = 0; t0 < sp.length; t0 += kTile, buffer ^= 1) {
-            const int64_t left = sp.length - t0;
-            float2 *steps = all_steps + buffer * kTile * H::CB;
-            float *proj = all_proj + buffer * 2 * kTile * H::SP;
+    if (!scans) {
+        // ---- moves tiles: at phase k it puts down tile k + 1, fetches tile k + 2, and sends off tile k - 1
+        const Share share(p.x.access, tid, channels);
+        const int slot0 = pair_slot<H::CB>(0, share.c);  // of an even step
+        float bias[Share::kPer];
 #pragma unroll
-            for (int i = 0; i < Tile::kPieces; ++i) {
-                int t, cc;
-                if (!Tile::place(p.x.access, i, t, cc)) continue;
-                float x[Tile::kPer], d[Tile::kPer];
-                next_x.open(i, x);
-                next_dt.open(i, d);
-                if (p.x.access == kTileSteps) {
-                    const float ba = p.dt_bias != nullptr && cc < channels ? load_one(p.dt_bias, c0 + cc, p.channels, 213) : 0.0f;
+        for (int e = 0; e < Share::kPer; ++e) {
+            const int ch = share.by_step ? share.c : share.c + e;
+            bias[e] = p.dt_bias != nullptr && ch < channels ? load_one(p.dt_bias, c0 + ch, p.channels, 213) : 0.0f;
+        }
+        for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
+            const Span sp = span_of(p.seq, s);
+            const int64_t tiles = (sp.length + kTile - 1) / kTile;
+            const auto left_at = [&](int64_t k) { return (int)(sp.length - k * kTile < kTile ? sp.length - k * kTile : kTile); };
+            int64_t at_x = share.offset(p.x, sp.row, c0, sp.start), at_dt = share.offset(p.dt, sp.row, c0, sp.start);
+            int64_t at_z = share.offset(p.z, sp.row, c0, sp.start), at_out = share.offset(p.out, sp.row, c0, sp.start);
+            uint4 next_x[Share::kPieces], next_dt[Share::kPieces], next_z[Share::kPieces];
+            Proj next_proj;
+            const auto fetch = [&](int64_t k) {
+                if (k >= tiles) return;
+                share.fetch(p.x, at_x, left_at(k), 215, next_x);
+                share.fetch(p.dt, at_dt, left_at(k), 216, next_dt);
+                next_proj.fetch(tid, p.B, p.C, sp.row, g, S, sp.start + k * kTile, left_at(k));
+                at_x += kTile * p.x.st;
+                at_dt += kTile * p.dt.st;
+            };
+            fetch(0);
+            int put_at = 0, send_at = 1;  // tiles k + 1 and k - 1 modulo 3
+            for (int64_t k = -1; k <= tiles; ++k) {
+                if (k + 1 < tiles) {
+                    const int left = left_at(k + 1);
+                    float2 *steps = all_steps + put_at * kTile * H::CB;
 #pragma unroll
-                    for (int k = 0; k < Tile::kPer; k += 2) {
-                        pair_t w = make_pair(d[k] + ba, d[k + 1] + ba);
-                        if (p.softplus) w = softplus2(w);
-                        const float2 f = halves(w);
-                        // behind the last step: decay 1, no input
-                        steps[pair_slot<H::CB>(t + k, cc)] = t + k < left ? make_float2(f.x, x[k]) : make_float2(0.0f, 0.0f);
-                        steps[pair_slot<H::CB>(t + k + 1, cc)] = t + k + 1 < left ? make_float2(f.y, x[k + 1]) : make_float2(0.0f, 0.0f);
+                    for (int i = 0; i < Share::kPieces; ++i) {
+                        const int t = share.t + i * share.next;
+                        float x[Share::kPer], d[Share::kPer];
+                        Share::open(next_x[i], x);
+                        Share::open(next_dt[i], d);
+#pragma unroll
+                        for (int e = 0; e < Share::kPer; ++e) {
+                            d[e] += bias[e];
+                            if (p.softplus) d[e] = softplus(d[e]);
+                            if ((share.by_step ? t + e : t) >= left) d[e] = x[e] = 0.0f;  // behind the last step: decay 1, no input
+                        }
+                        if (share.t >= kTile) continue;
+                        if (share.by_step) {
+#pragma unroll
+                            for (int e = 0; e < Share::kPer; ++e) steps[pair_slot<H::CB>(t + e, share.c)] = make_float2(d[e], x[e]);
+                        } else {
+                            // 8 adjacent channels are 4 units of 16 bytes whose order the step's parity turns
+                            float2 *to = steps + t * H::CB;
+#pragma unroll
+                            for (int e = 0; e < Share::kPer; e += 2)
+                                *reinterpret_cast<float4 *>(to + ((slot0 ^ e) ^ (2 * (t & 1)))) = make_float4(d[e], x[e], d[e + 1], x[e + 1]);
+                        }
                     }
-                } else {
-                    float bias[Tile::kPer];
+                    next_proj.put(tid, p.B.access, left, all_proj + ((k + 1) & 1) * 2 * kTile * H::SP);
+                    fetch(k + 2);
+                }
+                if (k >= 1) {
+                    const float2 *steps = all_steps + send_at * kTile * H::CB;
 #pragma unroll
-                    for (int k = 0; k < Tile::kPer; ++k)
-                        bias[k] = p.dt_bias != nullptr && cc + k < channels ? load_one(p.dt_bias, c0 + cc + k, p.channels, 213) : 0.0f;
+                    for (int i = 0; i < Share::kPieces; ++i) {
+                        const int t = share.t + i * share.next;
+                        if (share.t >= kTile) continue;
+                        float f[Share::kPer], z[Share::kPer];
+                        if (share.by_step) {
 #pragma unroll
-                    for (int k = 0; k < Tile::kPer; k += 2) {
-                        pair_t w = make_pair(d[k] + bias[k], d[k + 1] + bias[k + 1]);
-                        if (p.softplus) w = softplus2(w);
-                        const float2 f = halves(w);
-                        *reinterpret_cast<float4 *>(steps + pair_slot<H::CB>(t, cc + k)) =
-                            t < left ? make_float4(f.x, x[k], f.y, x[k + 1]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            for (int e = 0; e < Share::kPer; ++e) f[e] = steps[pair_slot<H::CB>(t + e, share.c)].x;
+                        } else {
+                            const float2 *from = steps + t * H::CB;
+#pragma unroll
+                            for (int e = 0; e < Share::kPer; e += 2) {
+                                const float4 w = *reinterpret_cast<const float4 *>(from + ((slot0 ^ e) ^ (2 * (t & 1))));
+                                f[e] = w.x;
+                                f[e + 1] = w.z;
+                            }
+                        }
+                        if (p.z.data != nullptr) {
+                            Share::open(next_z[i], z);
+#pragma unroll
+                            for (int e = 0; e < Share::kPer; ++e) f[e] *= z[e] * logistic(z[e]);
+                        }
+                        share.store(p.out, at_out, i, left_at(k - 1), 219, f);
                     }
+                    at_out += kTile * p.out.st;
                 }
-            }
-            next_proj.put(p.B.access, left, proj);
-            __syncthreads();
-            if (p.z.data != nullptr) next_z.fetch(p.z, sp.row, c0, channels, sp.start + t0, left, 218);
-            if (t0 + kTile < sp.length) fetch(t0 + kTile);
-            const int here = left < kTile ? ((int)left + kGroup - 1) / kGroup * kGroup : kTile;
-#pragma unroll 1
-            for (int t = 0; t < here; t += kGroup) {
-                if (p.checkpoints != nullptr && ((t0 + t) & ((1ll << p.tile_log2) - 1)) == 0)
-                    store_lane_states<SPL>(p.checkpoints, ((slot0 + ((t0 + t) >> p.tile_log2)) * p.channels + c) * S + q * SPL, have, p.vec,
-                                           p.checkpoint_slots * S * p.channels, 217, h);
-                float y[kGroup];
-#pragma unroll
-                for (int i = 0; i < kGroup; ++i) {
-                    const float2 dx = steps[pair_slot<H::CB>(t + i, cl)];
-                    pair_t b[SPL / 2], r[SPL / 2], sum = 0;
-                    load_lane_projection<SPL>(proj + (t + i) * H::SP + q * SPL, b);
-                    load_lane_projection<SPL>(proj + (kTile + t + i) * H::SP + q * SPL, r);
-                    const pair_t dt2 = both(dx.x), u2 = both(dx.x * dx.y);
-#pragma unroll
-                    for (int k = 0; k < SPL / 2; ++k) {
-                        h[k] = fma2(exp2_pair(mul2(dt2, A[k])), h[k], mul2(u2, b[k]));
-                        sum = fma2(h[k], r[k], sum);
-                    }
-                    const float2 f = halves(sum);
-                    y[i] = fmaf(D, dx.y, f.x + f.y);
+                if (p.z.data != nullptr && k >= 0 && k < tiles) {
+                    share.fetch(p.z, at_z, left_at(k), 218, next_z);
+                    at_z += kTile * p.z.st;
                 }
-                __syncwarp();  // the lanes of a channel have read the steps that are replaced
-                if constexpr (LN <= 4) {
-#pragma unroll
-                    for (int i = 0; i < kGroup; i += LN) {
-                        float v[LN];
-#pragma unroll
-                        for (int k = 0; k < LN; ++k) v[k] = y[i + k];
-                        steps[pair_slot<H::CB>(t + i + q, cl)].x = sum_and_spread<LN>(v, q);
-                    }
-                } else {
-                    steps[pair_slot<H::CB>(t + q, cl)].x = sum_and_spread<LN>(y, q);
-                }
-            }
-            __syncthreads();
-            // gate and store
-#pragma unroll
-            for (int i = 0; i < Tile::kPieces; ++i) {
-                int t, cc;
-                if (!Tile::place(p.out.access, i, t, cc)) continue;
-                float f[Tile::kPer], z[Tile::kPer];
-#pragma unroll
-                for (int k = 0; k < Tile::kPer; k += 2) {
-                    if (p.out.access == kTileSteps) {
-                        f[k] = steps[pair_slot<H::CB>(t + k, cc)].x;
-                        f[k + 1] = steps[pair_slot<H::CB>(t + k + 1, cc)].x;
-                    } else {
-                        const float4 w = *reinterpret_cast<const float4 *>(steps + pair_slot<H::CB>(t, cc + k));
-                        f[k] = w.x;
-                        f[k + 1] = w.z;
-                    }
-                }
-                if (p.z.data != nullptr) {
-                    next_z.open(i, z);
-#pragma unroll
-                    for (int k = 0; k < Tile::kPer; ++k) f[k] *= z[k] * logistic(z[k]);
-                }
-                Tile::store(p.out, sp.row, c0, channels, sp.start + t0, left, 219, t, cc, f);
+                put_at = put_at == 2 ? 0 : put_at + 1;
+                send_at = send_at == 2 ? 0 : send_at + 1;
+                __syncthreads();
             }
         }
-        if (p.state_out != nullptr) store_lane_states<SPL>(p.state_out, state_at, have, p.vec, state_extent, 220, h);
-        zero_uncovered<io_t>(p.seq, s, sp, p.out, c0, c0 + channels, 219);
-        __syncthreads();  // the last tile is no longer read
+    } else {
+        // ---- scans: at phase k tile k
+        const int lane = tid & 31, warp = tid >> 5;
+        const int q = lane % LN, cl = warp * H::DL + lane / LN;  // lanes of a channel are neighbours
+        const bool live = cl < channels;
+        const int64_t c = c0 + (live ? cl : 0);
+        const int have = live ? (S - q * SPL < SPL ? S - q * SPL : SPL) : 0;  // states of this lane (none: < 1)
+        pair_t A[SPL / 2];
+        load_lane_decays<SPL>(p.A, c * S + q * SPL, have, p.vec, p.channels * S, 261, A);
+        const float D = q == 0 && p.D != nullptr ? load_one(p.D, c, p.channels, 212) : 0.0f;
+        for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
+            const Span sp = span_of(p.seq, s);
+            const int64_t tiles = (sp.length + kTile - 1) / kTile;
+            const int64_t state_at = (s * p.channels + c) * S + q * SPL, state_extent = p.seq.count * p.channels * S;
+            pair_t h[SPL / 2] = {};
+            if (p.state != nullptr) load_lane_states<SPL>(p.state, state_at, have, p.vec, state_extent, 214, h);
+            const int64_t slot0 = p.checkpoints != nullptr ? checkpoint_base(p, s, sp.start) : 0;
+            int at = 0;  // tile k modulo 3
+            __syncthreads();  // phase -1
+            for (int64_t k = 0; k <= tiles; ++k) {
+                if (k < tiles) {
+                    float2 *steps = all_steps + at * kTile * H::CB;
+                    const float *proj = all_proj + (k & 1) * 2 * kTile * H::SP + q * SPL;
+                    const auto load = [&](int t, StepGroup<kAhead, SPL> &w) {
+#pragma unroll
+                        for (int i = 0; i < kAhead; ++i) {
+                            w.dx[i] = steps[pair_slot<H::CB>(t + i, cl)];
+                            load_lane_projection<SPL>(proj + (t + i) * H::SP, w.b[i]);
+                            load_lane_projection<SPL>(proj + (kTile + t + i) * H::SP, w.r[i]);
+                        }
+                    };
+                    // Sums of the group before are exchanged while the next group is worked on; their place is that of
+                    // steps which all lanes of the channel have loaded.
+                    const auto exchange = [&](int t, float (&y)[kGroup]) {
+                        constexpr int kSpread = LN < kGroup ? LN : kGroup;
+#pragma unroll
+                        for (int i = 0; i < kGroup; i += kSpread) {
+                            float v[kSpread];
+#pragma unroll
+                            for (int e = 0; e < kSpread; ++e) v[e] = y[i + e];
+                            const float sum = sum_and_spread<LN>(v, q);
+                            if (q < kSpread) steps[pair_slot<H::CB>(t + i + q, cl)].x = sum;
+                        }
+                    };
+                    const int64_t left = sp.length - k * kTile;
+                    const int here = left < kTile ? ((int)left + kGroup - 1) / kGroup * kGroup : kTile;
+                    StepGroup<kAhead, SPL> part[2];
+                    float y[kGroup], y_before[kGroup];
+                    load(0, part[0]);
+#pragma unroll 1
+                    for (int t = 0; t < here; t += kGroup) {
+                        if (p.checkpoints != nullptr && ((k * kTile + t) & ((1ll << p.tile_log2) - 1)) == 0)
+                            store_lane_states<SPL>(p.checkpoints, ((slot0 + ((k * kTile + t) >> p.tile_log2)) * p.channels + c) * S + q * SPL, have,
+                                                   p.vec, p.checkpoint_slots * S * p.channels, 217, h);
+#pragma unroll
+                        for (int i0 = 0; i0 < kGroup; i0 += kAhead) {
+                            const StepGroup<kAhead, SPL> &now = part[i0 / kAhead & 1];
+                            // the last part of a tile loads the first steps of no tile: any, and does not use them
+                            load((t + i0 + kAhead) & (kTile - 1), part[(i0 / kAhead + 1) & 1]);
+#pragma unroll
+                            for (int i = 0; i < kAhead; ++i) {
+                                pair_t sum;
+                                const pair_t dt2 = both(now.dx[i].x), u2 = both(now.dx[i].x * now.dx[i].y);
+#pragma unroll
+                                for (int e = 0; e < SPL / 2; ++e) {
+                                    h[e] = fma2(exp2_pair(mul2(dt2, A[e])), h[e], mul2(u2, now.b[i][e]));
+                                    sum = e == 0 ? mul2(h[e], now.r[i][e]) : fma2(h[e], now.r[i][e], sum);
+                                }
+                                const float2 f = halves(sum);
+                                y[i0 + i] = fmaf(D, now.dx[i].y, f.x + f.y);
+                            }
+                        }
+                        if (t > 0) exchange(t - kGroup, y_before);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < kGroup; ++i) y_before[i] = y[i];
+                    }
+                    exchange(here - kGroup, y_before);
+                }
+                at = at == 2 ? 0 : at + 1;
+                __syncthreads();
+            }
+            if (p.state_out != nullptr) store_lane_states<SPL>(p.state_out, state_at, have, p.vec, state_extent, 220, h);
+        }
     }
+    for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y)
+        zero_uncovered<io_t>(p.seq, s, span_of(p.seq, s), p.out, c0, c0 + channels, 219);
 }
 
 }  // namespace ssb

@@ -369,7 +369,7 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
             constexpr size_t smem = ssb::selective_lane_smem<LN, SPL>();
             if (int rc = allow_smem(kernel, smem)) return rc;
             const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)std::min<int64_t>(count, 65535));
-            kernel<<<grid, H::THREADS, smem, (cudaStream_t)stream>>>(a);
+            kernel<<<grid, 2 * H::THREADS, smem, (cudaStream_t)stream>>>(a);
             return check_launch("selective_lane_fwd_kernel");
         });
     });
