@@ -187,11 +187,11 @@ __device__ __forceinline__ float sum_and_spread(float (&v)[STEPS], int q) {
     return v[0];
 }
 
-template <int LN, int SPL>
+template <int LN, int SPL, int WARPS>
 struct LaneShape {
     static constexpr int SP = LN * SPL;                  // states, padded
     static constexpr int DL = 32 / LN;                   // channels of a warp
-    static constexpr int W = LN >= 16 ? 8 : 4;           // warps that scan, and as many that move tiles
+    static constexpr int W = WARPS;                      // warps that scan, and as many that move tiles
     static constexpr int CB = W * DL;                    // channels of a CTA
     static constexpr int THREADS = W * 32;               // of either kind
 };
@@ -204,9 +204,9 @@ __device__ __forceinline__ int pair_slot(int t, int c) {
     return t * CB + 2 * ((c >> 1) ^ ((c >> 3) & 3) ^ (t & 1)) + (c & 1);
 }
 
-template <int LN, int SPL>
+template <int LN, int SPL, int WARPS>
 __host__ __device__ constexpr size_t selective_lane_smem() {
-    using H = LaneShape<LN, SPL>;
+    using H = LaneShape<LN, SPL, WARPS>;
     return sizeof(float) * (size_t)(3 * 2 * kTile * H::CB + 2 * 2 * kTile * H::SP);  // three tiles of (dt, x), two of B and C
 }
 
@@ -278,9 +278,9 @@ struct StepGroup {
     pair_t b[STEPS][SPL / 2], r[STEPS][SPL / 2];
 };
 
-template <typename io_t, int LN, int SPL>
-__global__ void __launch_bounds__(2 * LaneShape<LN, SPL>::THREADS, LaneShape<LN, SPL>::W == 4 ? 2 : 1) selective_lane_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
-    using H = LaneShape<LN, SPL>;
+template <typename io_t, int LN, int SPL, int WARPS>
+__global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_fwd_kernel(const __grid_constant__ SelectiveArgs p) {
+    using H = LaneShape<LN, SPL, WARPS>;
     using Share = TileShare<io_t, H::CB, H::THREADS>;
     using Proj = ProjectionPieces<io_t, H::SP, H::THREADS>;
     constexpr int kGroup = 8;                      // steps whose sums are exchanged together

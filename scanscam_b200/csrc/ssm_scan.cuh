@@ -266,6 +266,25 @@ __device__ __forceinline__ void load8(const float *smem, float (&v)[kRun]) {
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
 }
 
+// N adjacent floats in shared memory, 16 (8) bytes at a time.
+template <int N>
+__device__ __forceinline__ void add_to(float *to, const float *v) {
+    if constexpr (N >= 4) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            float4 f = *reinterpret_cast<float4 *>(to + i);
+            f.x += v[i]; f.y += v[i + 1]; f.z += v[i + 2]; f.w += v[i + 3];
+            *reinterpret_cast<float4 *>(to + i) = f;
+        }
+    } else if constexpr (N == 2) {
+        float2 f = *reinterpret_cast<float2 *>(to);
+        f.x += v[0]; f.y += v[1];
+        *reinterpret_cast<float2 *>(to) = f;
+    } else {
+        *to += *v;
+    }
+}
+
 template <int TL, int W>
 struct ScanShape {
     static constexpr int DL = 32 / TL;       // lanes across channels
@@ -365,6 +384,7 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                 through[k] = 0;
                 bydecay[k] = 0;
             }
+            const pair_t span = add2(add2(add2(dt[0], dt[1]), add2(dt[2], dt[3])), add2(add2(dt[4], dt[5]), add2(dt[6], dt[7])));
             for (int n0 = 0; n0 < S; n0 += slab) {
                 const int count = S - n0 < slab ? S - n0 : slab;
                 Pieces next_B, next_C;
@@ -399,12 +419,9 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                         load8(Cs + n * H::PAD + tl * kRun, cv);
 #pragma unroll
                         for (int k = 0; k < kRun; ++k) a[k] = exp2_pair(mul2(dt[k], A));
-                        pair_t P = a[0], F = mul2(u[0], both(bv[0]));
+                        pair_t P = exp2_pair(mul2(span, A)), F = mul2(u[0], both(bv[0]));  // P: the decay over all 8 steps
 #pragma unroll
-                        for (int k = 1; k < kRun; ++k) {
-                            F = fma2(u[k], both(bv[k]), mul2(a[k], F));
-                            P = mul2(P, a[k]);
-                        }
+                        for (int k = 1; k < kRun; ++k) F = fma2(u[k], both(bv[k]), mul2(a[k], F));
                         const pair_t P0 = P;
                         compose_left<TL>(P, F, tl);
                         pair_t h = shfl_up2(fma2(P, h_in, F), H::DL);
@@ -464,12 +481,12 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                                 }
                             }
                         }
-                        constexpr int kHeld = 2 * kRun / H::DL;
-#pragma unroll
-                        for (int i = 0; i < kHeld; ++i) {
-                            const int w = at + i;
-                            float *to = (w < kRun ? sumB : sumC) + n * H::PAD + tl * kRun + (w & (kRun - 1));
-                            *to += v[i];
+                        constexpr int kHeld = 2 * kRun / H::DL;  // sums that this lane is left with: adjacent steps of B or of C
+                        if constexpr (kHeld == 2 * kRun) {
+                            add_to<kRun>(sumB + n * H::PAD + tl * kRun, v);
+                            add_to<kRun>(sumC + n * H::PAD + tl * kRun, v + kRun);
+                        } else {
+                            add_to<kHeld>((at < kRun ? sumB : sumC) + n * H::PAD + tl * kRun + (at & (kRun - 1)), v);
                         }
                     }
                     __syncthreads();

@@ -101,18 +101,30 @@ int allow_smem(K kernel, size_t bytes) {
 }
 
 // ---- selective scan -----------------------------------------------------------------------------
-constexpr int kBwdWarps = 8;
+#ifndef BW
+#define BW 4
+#endif
+#ifndef BWANT
+#define BWANT 1.5
+#endif
+constexpr int kBwdWarps = BW;
 
-// Calls f with the lanes that share a channel and the states each of them holds.
+// Calls f with the lanes that share a channel, the states each of them holds, and the warps of a CTA
+// that scan.  `eight`: 8 states a lane instead of 4, which leaves half the warps.
 template <typename F>
-auto with_lanes(int64_t states, F &&f) {
+auto with_lanes(int64_t states, bool eight, F &&f) {
     using std::integral_constant;
-    if (states <= 8) return f(integral_constant<int, 2>{}, integral_constant<int, 4>{});
-    if (states <= 16) return f(integral_constant<int, 4>{}, integral_constant<int, 4>{});
-    if (states <= 32) return f(integral_constant<int, 8>{}, integral_constant<int, 4>{});
-    if (states <= 64) return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-    if (states <= 128) return f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
-    return f(integral_constant<int, 32>{}, integral_constant<int, 8>{});
+    const integral_constant<int, 2> two;
+    const integral_constant<int, 4> four;
+    const integral_constant<int, 8> each8;
+    const integral_constant<int, 16> sixteen;
+    const integral_constant<int, 32> all;
+    if (states <= 8) return f(two, four, four);
+    if (states <= 16) return eight ? f(two, each8, four) : f(four, four, four);
+    if (states <= 32) return eight ? f(four, each8, four) : f(each8, four, four);
+    if (states <= 64) return eight ? f(each8, each8, four) : f(sixteen, four, four);
+    if (states <= 128) return eight ? f(sixteen, each8, four) : f(all, four, each8);
+    return f(all, each8, each8);
 }
 
 // Calls f with the split of a warp between time and channels as a compile-time constant.
@@ -141,7 +153,7 @@ size_t smem_of(int tl, int64_t states) {  // the largest of any type
 // Lanes across time: the fewest (they cost shuffles) that give every SM a CTA.
 int split_of(int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
     for (int tl = 4; tl < 32; tl *= 2)
-        if (groups * channel_blocks(per_group, tl, kBwdWarps) * std::max<int64_t>(sequences, 1) >= (int64_t)sm_count() &&
+        if (groups * channel_blocks(per_group, tl, kBwdWarps) * std::max<int64_t>(sequences, 1) >= BWANT * sm_count() &&
             smem_of(tl, states) <= kSmemLimit)
             return tl;
     return 32;
@@ -358,15 +370,19 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
         if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
     return with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
-        return with_lanes(p->states, [&](auto lanes, auto each) {
-            constexpr int LN = decltype(lanes)::value, SPL = decltype(each)::value;
-            using H = ssb::LaneShape<LN, SPL>;
-            const int64_t per_group = p->channels / p->groups;
+        const int64_t per_group = p->channels / p->groups;
+        // 8 states a lane need 5 instructions an exponential where 4 need 8, but a warp alone on its scheduler takes
+        // as long for either: from two warps a scheduler up (13 prompts of 4096 channels, 16 states: 136 us against
+        // 169; [4, 2048, 2048], half a warp a scheduler: 179 against 177; [1, 2048, 8192]: 636 against 505).
+        const bool eight = p->channels * count * ((p->states + 7) / 8) >= 2 * 4 * 32 * (int64_t)sm_count();
+        return with_lanes(p->states, eight, [&](auto lanes, auto each, auto warps) {
+            constexpr int LN = decltype(lanes)::value, SPL = decltype(each)::value, W = decltype(warps)::value;
+            using H = ssb::LaneShape<LN, SPL, W>;
             ssb::SelectiveArgs a = selective_args(p, (per_group + H::CB - 1) / H::CB);
             a.x.access = a.dt.access = a.z.access = a.out.access = tile_access(p);
             if (a.B.access != a.C.access) a.B.access = a.C.access = ssb::kProjAny;
-            auto kernel = ssb::selective_lane_fwd_kernel<io_t, LN, SPL>;
-            constexpr size_t smem = ssb::selective_lane_smem<LN, SPL>();
+            auto kernel = ssb::selective_lane_fwd_kernel<io_t, LN, SPL, W>;
+            constexpr size_t smem = ssb::selective_lane_smem<LN, SPL, W>();
             if (int rc = allow_smem(kernel, smem)) return rc;
             const dim3 grid((unsigned)(a.blocks_per_group * p->groups), (unsigned)std::min<int64_t>(count, 65535));
             kernel<<<grid, 2 * H::THREADS, smem, (cudaStream_t)stream>>>(a);
