@@ -104,17 +104,22 @@ __device__ __forceinline__ float relu_or_nan(float v) {
 // atanh(s) = s + s q P(q), q = s^2, where P is a cubic fitted (Chebyshev, weighted with q) to
 // (atanh(s) / s - 1) / q on [0, 1/9]: 4.6e-9 of the value.  Below -87 the result stays at e^-87 = 1.6e-38,
 // where the type's normal range ends.  The exponential as in exp_accurate.
-__device__ __forceinline__ float softplus(float v) {
+__device__ __forceinline__ float softplus_and_slope(float v, float &slope) {  // the slope is 1 / (1 + e^-v)
     const float x = fmaxf(-fabsf(v), -87.0f);
     const float hi = x * kLog2e;
     const float lo = fmaf(x, 1.925963033500945e-8f, fmaf(x, kLog2e, -hi));
     float e = exp2_approx(hi);
     e = fmaf(e, lo * kLn2, e);
+    slope = (v < 0.0f ? e : 1.0f) * reciprocal_approx(1.0f + e);
     const float s = e * reciprocal_approx(e + 2.0f), q = s * s;
     float p = fmaf(q, 0.13988047f, 0.14004979f);
     p = fmaf(p, q, 0.20010476f);
     p = fmaf(p, q, 0.33333215f);
     return fmaf(fmaf(p * q, s, s), 2.0f, relu_or_nan(v));
+}
+__device__ __forceinline__ float softplus(float v) {
+    float slope;
+    return softplus_and_slope(v, slope);
 }
 __device__ __forceinline__ pair_t softplus2(pair_t v) {
     const float2 f = halves(v);

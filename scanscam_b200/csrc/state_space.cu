@@ -9,6 +9,7 @@
 
 #include "host_common.h"
 #include "short_conv.cuh"
+#include "ssm_backward.cuh"
 #include "ssm_forward.cuh"
 #include "ssm_scan.cuh"
 #include "ssm_step.cuh"
@@ -19,7 +20,7 @@ using ssb_host::sm_count;
 
 namespace {
 
-constexpr int64_t kMaxStates = 256;
+constexpr int64_t kMaxStates = 256, kLaneBackwardStates = 32;
 constexpr size_t kSmemLimit = 227 * 1024;
 
 size_t size_of(int dtype) { return dtype == SSB_F32 ? 4 : 2; }
@@ -101,13 +102,7 @@ int allow_smem(K kernel, size_t bytes) {
 }
 
 // ---- selective scan -----------------------------------------------------------------------------
-#ifndef BW
-#define BW 4
-#endif
-#ifndef BWANT
-#define BWANT 1.5
-#endif
-constexpr int kBwdWarps = BW;
+constexpr int kBwdWarps = 4, kLaneWarps = 4;
 
 // Calls f with the lanes that share a channel, the states each of them holds, and the warps of a CTA
 // that scan.  `eight`: 8 states a lane instead of 4, which leaves half the warps.
@@ -150,10 +145,10 @@ size_t smem_of(int tl, int64_t states) {  // the largest of any type
     });
 }
 
-// Lanes across time: the fewest (they cost shuffles) that give every SM a CTA.
+// Lanes across time: the fewest (they cost shuffles) that give the SMs three CTAs for two.
 int split_of(int64_t per_group, int64_t groups, int64_t sequences, int64_t states) {
     for (int tl = 4; tl < 32; tl *= 2)
-        if (groups * channel_blocks(per_group, tl, kBwdWarps) * std::max<int64_t>(sequences, 1) >= BWANT * sm_count() &&
+        if (groups * channel_blocks(per_group, tl, kBwdWarps) * std::max<int64_t>(sequences, 1) * 2 >= 3 * sm_count() &&
             smem_of(tl, states) <= kSmemLimit)
             return tl;
     return 32;
@@ -182,20 +177,33 @@ int check_selective(const ssb_selective_t *p, bool data) {
 
 int64_t count_of(const ssb_selective_t *p) { return p->offsets != nullptr ? p->sequences : p->batch; }
 
-int backward_split(const ssb_selective_t *p) {
-    return split_of(p->channels / p->groups, p->groups, count_of(p), p->states);
+// The backward's shape.  Up to 32 states: lanes across states (ssm_backward.cuh); the sums of B and C that its
+// warps keep in shared memory grow with the states, so beyond that lanes across time (ssm_scan.cuh).
+struct BackwardForm {
+    bool lanes;
+    int split;             // lanes across time of the other form
+    int64_t tile, blocks;  // steps between checkpoints; channel blocks of a group
+};
+BackwardForm backward_form(const ssb_selective_t *p) {
+    const int64_t per_group = p->channels / p->groups;
+    if (p->states <= kLaneBackwardStates) {
+        const int64_t cb = kLaneWarps * 32 / (p->states <= 8 ? 2 : p->states <= 16 ? 4 : 8);
+        return {true, 0, ssb::kCheckpointSteps, (per_group + cb - 1) / cb};
+    }
+    const int tl = split_of(per_group, p->groups, count_of(p), p->states);
+    return {false, tl, tl * ssb::kRun, channel_blocks(per_group, tl, kBwdWarps)};
 }
 int64_t checkpoint_slots(const ssb_selective_t *p) {
-    const int64_t tile = backward_split(p) * ssb::kRun;
+    const int64_t tile = backward_form(p).tile;
     return p->offsets != nullptr ? p->steps / tile + p->sequences + 1 : p->batch * ((p->steps + tile - 1) / tile);
 }
 
-// How pieces of all the forward's [N, C, T] operands may be fetched: the same way for each of them.
-int tile_access(const ssb_selective_t *p) {
+// How pieces of all [N, C, T] operands of a kernel may be fetched: the same way for each of them.
+int tile_access(const ssb_selective_t *p, std::initializer_list<const ssb_view_t *> views) {
     const int64_t per = 16 / (int64_t)size_of(p->dtype);
     bool channels = p->groups == 1 || p->channels / p->groups % per == 0;  // blocks of channels start at whole pieces
     bool steps = p->offsets == nullptr && p->steps % per == 0;
-    for (const ssb_view_t *v : {&p->x, &p->dt, &p->z, &p->out}) {
+    for (const ssb_view_t *v : views) {
         if (v->data == nullptr) continue;
         const bool base = aligned(v->data, 16) && v->stride[0] % per == 0;
         channels = channels && base && v->stride[1] == 1 && v->stride[2] % per == 0;
@@ -230,14 +238,14 @@ ssb::SelectiveArgs selective_args(const ssb_selective_t *p, int64_t blocks_per_g
     a.checkpoints = p->checkpoints;
     if (p->checkpoints != nullptr) {
         a.checkpoint_slots = checkpoint_slots(p);
-        for (a.tile_log2 = 3; (1 << a.tile_log2) < backward_split(p) * ssb::kRun;) ++a.tile_log2;
+        for (a.tile_log2 = 3; (1 << a.tile_log2) < backward_form(p).tile;) ++a.tile_log2;
     }
     return a;
 }
 
 // CTAs that share the sequences of one channel block in the backward: each keeps one set of sums for A, D and dt_bias.
 int64_t backward_rows(const ssb_selective_t *p) {
-    const int64_t blocks = p->groups * channel_blocks(p->channels / p->groups, backward_split(p), kBwdWarps);
+    const int64_t blocks = p->groups * backward_form(p).blocks;
     const int64_t want = std::max<int64_t>(1, (4 * (int64_t)sm_count() + blocks - 1) / std::max<int64_t>(blocks, 1));
     return std::max<int64_t>(1, std::min(count_of(p), want));
 }
@@ -249,7 +257,7 @@ struct BackwardParts {
 };
 BackwardParts backward_parts(const ssb_selective_t *p) {
     return {p->batch * p->steps * p->groups * p->states, p->channels * p->states, p->channels,
-            channel_blocks(p->channels / p->groups, backward_split(p), kBwdWarps), backward_rows(p)};
+            backward_form(p).blocks, backward_rows(p)};
 }
 
 // ---- short convolution ----------------------------------------------------------------------------
@@ -379,7 +387,7 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
             constexpr int LN = decltype(lanes)::value, SPL = decltype(each)::value, W = decltype(warps)::value;
             using H = ssb::LaneShape<LN, SPL, W>;
             ssb::SelectiveArgs a = selective_args(p, (per_group + H::CB - 1) / H::CB);
-            a.x.access = a.dt.access = a.z.access = a.out.access = tile_access(p);
+            a.x.access = a.dt.access = a.z.access = a.out.access = tile_access(p, {&p->x, &p->dt, &p->z, &p->out});
             if (a.B.access != a.C.access) a.B.access = a.C.access = ssb::kProjAny;
             auto kernel = ssb::selective_lane_fwd_kernel<io_t, LN, SPL, W>;
             constexpr size_t smem = ssb::selective_lane_smem<LN, SPL, W>();
@@ -422,17 +430,40 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
     q.gz = view3(g->gz, p->dtype, p->batch, p->channels, p->steps, from_zero, even);
     q.gstate_out = g->gstate_out;
     q.gstate = g->gstate;
-    q.part_B = part;
-    q.part_C = q.part_B + parts.parts_proj * parts.proj;
-    q.part_A = q.part_C + parts.parts_proj * parts.proj;
+    q.part_A = part;
     q.part_D = q.part_A + parts.parts_seq * parts.A;
     q.part_bias = q.part_D + parts.parts_seq * parts.channel;
+    q.part_B = q.part_bias + parts.parts_seq * parts.channel;
+    q.part_C = q.part_B + parts.parts_proj * parts.proj;
     q.rows = p->batch;
+    const BackwardForm form = backward_form(p);
     const int rc = with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
-        return with_split(backward_split(p), [&](auto k) {
+        if (form.lanes) {
+            const auto launch = [&](auto lanes) {
+                constexpr int LN = decltype(lanes)::value;
+                using H = ssb::LaneShape<LN, 4, kLaneWarps>;
+                ssb::SelectiveArgs a = selective_args(p, form.blocks);
+                ssb::SelectiveGradArgs b = q;
+                a.vec = a.vec && aligned(q.gstate_out, 16) && aligned(q.gstate, 16) && aligned(q.part_A, 16) && aligned(q.part_B, 16) && aligned(q.part_C, 16);
+                a.x.access = a.dt.access = a.z.access = b.gout.access = b.gx.access = b.gdt.access = b.gz.access =
+                    tile_access(p, {&p->x, &p->dt, &p->z, &g->gout, &g->gx, &g->gdt, p->z.data != nullptr ? &g->gz : &p->z});
+                if (a.B.access != a.C.access) a.B.access = a.C.access = ssb::kProjAny;
+                auto kernel = ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>;
+                constexpr size_t smem = ssb::selective_lane_bwd_smem<io_t, LN, kLaneWarps>();
+                if (int bad = allow_smem(kernel, smem)) return bad;
+                const dim3 grid((unsigned)(form.blocks * p->groups), (unsigned)parts.parts_seq);
+                kernel<<<grid, 2 * H::THREADS, smem, (cudaStream_t)stream>>>(a, b);
+                return check_launch("selective_lane_bwd_kernel");
+            };
+            using std::integral_constant;
+            if (p->states <= 8) return launch(integral_constant<int, 2>{});
+            if (p->states <= 16) return launch(integral_constant<int, 4>{});
+            return launch(integral_constant<int, 8>{});
+        }
+        return with_split(form.split, [&](auto k) {
             constexpr int TL = decltype(k)::value;
-            const ssb::SelectiveArgs a = selective_args(p, channel_blocks(p->channels / p->groups, TL, kBwdWarps));
+            const ssb::SelectiveArgs a = selective_args(p, form.blocks);
             auto kernel = ssb::selective_bwd_kernel<io_t, TL, kBwdWarps>;
             const size_t smem = ssb::selective_bwd_smem<io_t, TL, kBwdWarps>(p->states);
             if (int bad = allow_smem(kernel, smem)) return bad;
