@@ -20,6 +20,15 @@ namespace ssb {
 
 constexpr int kCheckpointSteps = 16;
 
+// Registers of a thread at launch, and after the two kinds of warps have parted (one warpgroup of 4 warps each):
+// what the ones give up the others take, so the sum never exceeds the launch's.
+constexpr int kLaunchRegisters = 128, kScanRegisters = 152, kMoveRegisters = 104;
+static_assert(kScanRegisters + kMoveRegisters <= 2 * kLaunchRegisters, "a block's registers are what it was launched with");
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <typename io_t, int LN, int WARPS>
 __host__ __device__ constexpr size_t selective_lane_bwd_smem() {
     using H = LaneShape<LN, 4, WARPS>;
@@ -85,6 +94,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
     __syncthreads();
 
     if (!scans) {
+        registers_down<kMoveRegisters>();
         const Share share(p.x.access, tid, channels);
         const int slot0 = pair_slot<H::CB>(0, share.c);
         float gD[kPer], gbias[kPer];
@@ -281,6 +291,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
             mine_b[e] = share.works ? gbias[e] : 0.0f;
         }
     } else {
+        registers_up<kScanRegisters>();
         const int lane = tid & 31, warp = tid >> 5;
         const int ql = lane % LN, r = lane / LN, cl = warp * H::DL + r;
         const bool live = cl < channels;
@@ -311,15 +322,13 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
                     const float *Bs = all_proj + (phase & 1) * 2 * kTile * H::SP + ql * SPL, *Cs = Bs + kTile * H::SP;
                     float *sums = all_sums + ((phase & 1) * WARPS + warp) * kTile * 2 * H::SP + ql * SPL;
                     // two steps' 8 sums over the warp's channels, into the rows of B (0) or C (1)
-                    const auto send_sums = [&](float (&v)[8], int t, int which) {
-                        const int i = sum_over_channels<H::DL, LN>(v, r);
+                    const auto send_sums = [&](float (&v)[8], int i, int t, int which) {
                         float *to = sums + ((t + (i >> 2)) * 2 + which) * H::SP + (i & 3);
                         if constexpr (H::DL >= 8) {
                             if (r < 8) *to = v[0];
-                        } else if constexpr (H::DL == 4) {
-                            *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
                         } else {
-                            *reinterpret_cast<float4 *>(to) = make_float4(v[0], v[1], v[2], v[3]);
+                            static_assert(H::DL == 4, "two sums a lane");
+                            *reinterpret_cast<float2 *>(to) = make_float2(v[0], v[1]);
                         }
                     };
 #pragma unroll 1
@@ -347,58 +356,63 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
 #pragma unroll
                         for (int sub = 3; sub >= 0; --sub) {
                             const int t4 = t16 + sub * 4;
-                            pair_t h[2] = {start[sub][0], start[sub][1]}, a[4][2], m[4][2];
+                            pair_t h[2] = {start[sub][0], start[sub][1]}, a[4][2], m[4][2], b[4][2], cc[4][2];
                             float2 dx[4];
-                            float gy[4], y[4], v[8];
+                            float gy[4], y[4], vB[2][8], vC[2][8];
+                            // everything these steps need is loaded before anything is stored
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 dx[i] = steps[pair_slot<H::CB>(t4 + i, cl)];
                                 gy[i] = gys[(t4 + i) * H::CB];
+                                load_lane_projection<SPL>(Bs + (t4 + i) * H::SP, b[i]);
+                                load_lane_projection<SPL>(Cs + (t4 + i) * H::SP, cc[i]);
                             }
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const pair_t dt2 = both(dx[i].x), u2 = both(dx[i].x * dx[i].y), gy2 = both(gy[i]);
-                                pair_t b[2], cc[2], sum;
-                                load_lane_projection<SPL>(Bs + (t4 + i) * H::SP, b);
-                                load_lane_projection<SPL>(Cs + (t4 + i) * H::SP, cc);
+                                pair_t sum;
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
                                     a[i][e] = exp2_pair(mul2(dt2, A[e]));
                                     m[i][e] = mul2(a[i][e], h[e]);  // a_t h_{t-1}
-                                    h[e] = fma2(u2, b[e], m[i][e]);
-                                    sum = e == 0 ? mul2(h[e], cc[e]) : fma2(h[e], cc[e], sum);
+                                    h[e] = fma2(u2, b[i][e], m[i][e]);
+                                    sum = e == 0 ? mul2(h[e], cc[i][e]) : fma2(h[e], cc[i][e], sum);
                                     const float2 f = halves(mul2(gy2, h[e]));
-                                    v[(i & 1) * 4 + 2 * e] = f.x;
-                                    v[(i & 1) * 4 + 2 * e + 1] = f.y;
+                                    vC[i >> 1][(i & 1) * 4 + 2 * e] = f.x;
+                                    vC[i >> 1][(i & 1) * 4 + 2 * e + 1] = f.y;
                                 }
                                 const float2 f = halves(sum);
                                 y[i] = f.x + f.y;
-                                if (i & 1) send_sums(v, t4 + i - 1, 1);
                             }
                             float through[4], bydecay[4];
 #pragma unroll
                             for (int i = 3; i >= 0; --i) {
                                 const pair_t dt2 = both(dx[i].x), u2 = both(dx[i].x * dx[i].y), gy2 = both(gy[i]);
-                                pair_t b[2], cc[2], sum_b, sum_a;
-                                load_lane_projection<SPL>(Bs + (t4 + i) * H::SP, b);
-                                load_lane_projection<SPL>(Cs + (t4 + i) * H::SP, cc);
+                                pair_t sum_b, sum_a;
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    const pair_t dh = fma2(gy2, cc[e], adjoint[e]);
+                                    const pair_t dh = fma2(gy2, cc[i][e], adjoint[e]);
                                     adjoint[e] = mul2(a[i][e], dh);
                                     const pair_t w = mul2(dh, m[i][e]);
-                                    sum_b = e == 0 ? mul2(dh, b[e]) : fma2(dh, b[e], sum_b);
+                                    sum_b = e == 0 ? mul2(dh, b[i][e]) : fma2(dh, b[i][e], sum_b);
                                     sum_a = e == 0 ? mul2(w, A[e]) : fma2(w, A[e], sum_a);
                                     dA[e] = fma2(w, dt2, dA[e]);
                                     const float2 f = halves(mul2(dh, u2));
-                                    v[(i & 1) * 4 + 2 * e] = f.x;
-                                    v[(i & 1) * 4 + 2 * e + 1] = f.y;
+                                    vB[i >> 1][(i & 1) * 4 + 2 * e] = f.x;
+                                    vB[i >> 1][(i & 1) * 4 + 2 * e + 1] = f.y;
                                 }
                                 const float2 f = halves(sum_b), o = halves(sum_a);
                                 through[i] = f.x + f.y;
                                 bydecay[i] = o.x + o.y;
-                                if (!(i & 1)) send_sums(v, t4 + i, 0);
                             }
+                            // independent exchanges, then the stores
+                            const int i0 = sum_over_channels<H::DL, LN>(vC[0], r), i1 = sum_over_channels<H::DL, LN>(vC[1], r);
+                            sum_over_channels<H::DL, LN>(vB[0], r);
+                            sum_over_channels<H::DL, LN>(vB[1], r);
+                            send_sums(vC[0], i0, t4, 1);
+                            send_sums(vC[1], i1, t4 + 2, 1);
+                            send_sums(vB[0], i0, t4, 0);
+                            send_sums(vB[1], i1, t4 + 2, 0);
                             // the channel's sums take the place of the steps, which all its lanes have read
                             __syncwarp();
                             constexpr int kSpread = LN < 4 ? LN : 4;

@@ -101,6 +101,17 @@ int allow_smem(K kernel, size_t bytes) {
     return e == cudaSuccess ? SSB_OK : fail(SSB_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
 }
 
+// A kernel whose warps pass registers to one another has to be launched with as many as they will hold in all,
+// or those that ask for more wait for good.
+template <auto kKernel>
+int check_registers() {
+    static const int registers = [] {
+        cudaFuncAttributes a;
+        return cudaFuncGetAttributes(&a, kKernel) == cudaSuccess ? a.numRegs : -1;
+    }();
+    return registers == ssb::kLaunchRegisters ? SSB_OK : fail(SSB_ERR_LAUNCH, "kernel built with %d registers, not %d", registers, ssb::kLaunchRegisters);
+}
+
 // ---- selective scan -----------------------------------------------------------------------------
 constexpr int kBwdWarps = 4, kLaneWarps = 4;
 
@@ -177,8 +188,10 @@ int check_selective(const ssb_selective_t *p, bool data) {
 
 int64_t count_of(const ssb_selective_t *p) { return p->offsets != nullptr ? p->sequences : p->batch; }
 
-// The backward's shape.  Up to 32 states: lanes across states (ssm_backward.cuh); the sums of B and C that its
-// warps keep in shared memory grow with the states, so beyond that lanes across time (ssm_scan.cuh).
+// The backward's shape.  Up to 32 states and with a warp for most schedulers: lanes across states
+// (ssm_backward.cuh; [4, 2048, 2048], 16 states: 469 us against 699).  The sums of B and C that its warps keep in
+// shared memory grow with the states, and a warp walks all steps of its sequence, so else lanes across time
+// (ssm_scan.cuh; [2, 1024, 1024], 64 states: 423 us against 703; [2, 387, 1001], 10 states: 106 us against 166).
 struct BackwardForm {
     bool lanes;
     int split;             // lanes across time of the other form
@@ -186,7 +199,7 @@ struct BackwardForm {
 };
 BackwardForm backward_form(const ssb_selective_t *p) {
     const int64_t per_group = p->channels / p->groups;
-    if (p->states <= kLaneBackwardStates) {
+    if (p->states <= kLaneBackwardStates && p->channels * count_of(p) * ((p->states + 3) / 4) >= 4 * 32 * (int64_t)sm_count()) {
         const int64_t cb = kLaneWarps * 32 / (p->states <= 8 ? 2 : p->states <= 16 ? 4 : 8);
         return {true, 0, ssb::kCheckpointSteps, (per_group + cb - 1) / cb};
     }
@@ -452,6 +465,7 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
                 auto kernel = ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>;
                 constexpr size_t smem = ssb::selective_lane_bwd_smem<io_t, LN, kLaneWarps>();
                 if (int bad = allow_smem(kernel, smem)) return bad;
+                if (int bad = check_registers<ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>>()) return bad;
                 const dim3 grid((unsigned)(form.blocks * p->groups), (unsigned)parts.parts_seq);
                 kernel<<<grid, 2 * H::THREADS, smem, (cudaStream_t)stream>>>(a, b);
                 return check_launch("selective_lane_bwd_kernel");
