@@ -47,53 +47,88 @@ __device__ __forceinline__ int64_t find_sequence(const Sequences &q, int64_t t, 
     return lo;
 }
 
+// V adjacent channels of one step (4 or 1), as fetched and as pairs.
 template <typename io_t, int V>
 struct Lump {
-    float v[V];
+    static constexpr int kPairs = (V + 1) / 2, kWords = V == 1 ? 1 : V * (int)sizeof(io_t) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void open(pair_t (&f)[kPairs]) const {
+        if constexpr (V == 1) {
+            float v;
+            if constexpr (sizeof(io_t) == 4) {
+                v = __uint_as_float(w[0]);
+            } else {
+                float unused;
+                unpack2<io_t>(w[0], v, unused);
+            }
+            f[0] = make_pair(v, 0.0f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                if constexpr (sizeof(io_t) == 4) {
+                    f[i] = make_pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+                } else {
+                    float lo, hi;
+                    unpack2<io_t>(w[i], lo, hi);
+                    f[i] = make_pair(lo, hi);
+                }
+            }
+        }
+    }
 };
 template <typename io_t, int V>
-__device__ __forceinline__ Lump<io_t, V> load_lump(const View3 &w, int64_t at, int site) {
+__device__ __forceinline__ Lump<io_t, V> load_lump(const View3 &v, int64_t at, int site) {
     Lump<io_t, V> r;
-    const io_t *p = static_cast<const io_t *>(w.data) + at;
+    const io_t *p = static_cast<const io_t *>(v.data) + at;
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = 0.0f;
-    if (!SSB_VECTOR_OK(p, V * (int)sizeof(io_t), at + V - 1, w.extent, site)) return r;
+    for (int i = 0; i < Lump<io_t, V>::kWords; ++i) r.w[i] = 0;
+    if (!SSB_VECTOR_OK(p, V * (int)sizeof(io_t), at + V - 1, v.extent, site)) return r;
     if constexpr (V == 1) {
-        r.v[0] = static_cast<float>(*p);
+        if constexpr (sizeof(io_t) == 4) r.w[0] = *reinterpret_cast<const uint32_t *>(p);
+        else r.w[0] = *reinterpret_cast<const uint16_t *>(p);
     } else if constexpr (sizeof(io_t) == 4) {
-        static_assert(V == 4, "16-byte accesses");
-        const float4 f = *reinterpret_cast<const float4 *>(p);
-        r.v[0] = f.x; r.v[1] = f.y; r.v[2] = f.z; r.v[3] = f.w;
+        const uint4 f = *reinterpret_cast<const uint4 *>(p);
+        r.w[0] = f.x; r.w[1] = f.y; r.w[2] = f.z; r.w[3] = f.w;
     } else {
-        static_assert(V == 4, "8-byte accesses");
         const uint2 f = *reinterpret_cast<const uint2 *>(p);
-        unpack2<io_t>(f.x, r.v[0], r.v[1]);
-        unpack2<io_t>(f.y, r.v[2], r.v[3]);
+        r.w[0] = f.x; r.w[1] = f.y;
     }
     return r;
 }
 template <typename io_t, int V>
-__device__ __forceinline__ void store_lump(const View3 &w, int64_t at, int site, const float (&v)[V]) {
-    io_t *p = static_cast<io_t *>(w.data) + at;
-    if (!SSB_VECTOR_OK(p, V * (int)sizeof(io_t), at + V - 1, w.extent, site)) return;
-    if constexpr (V == 1) *p = static_cast<io_t>(v[0]);
-    else if constexpr (sizeof(io_t) == 4) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<io_t>(v[0], v[1]), pack2<io_t>(v[2], v[3]));
+__device__ __forceinline__ void store_lump(const View3 &v, int64_t at, int site, const pair_t (&f)[(V + 1) / 2]) {
+    io_t *p = static_cast<io_t *>(v.data) + at;
+    if (!SSB_VECTOR_OK(p, V * (int)sizeof(io_t), at + V - 1, v.extent, site)) return;
+    const float2 a = halves(f[0]);
+    if constexpr (V == 1) {
+        *p = static_cast<io_t>(a.x);
+    } else {
+        const float2 b = halves(f[1]);
+        if constexpr (sizeof(io_t) == 4) *reinterpret_cast<float4 *>(p) = make_float4(a.x, a.y, b.x, b.y);
+        else *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<io_t>(a.x, a.y), pack2<io_t>(b.x, b.y));
+    }
+}
+// channel i of V
+template <int N>
+__device__ __forceinline__ float channel_of(const pair_t (&f)[N], int i) {
+    const float2 h = halves(f[i / 2]);
+    return i & 1 ? h.y : h.x;
 }
 
 // Step `pos` (relative to the sequence's start; below zero: in the carried window) of V channels.
 template <typename io_t, int V, int W>
-__device__ __forceinline__ void input_at(const ConvArgs &p, const Span &sp, int64_t s, int64_t pos, int64_t c, float (&r)[V]) {
+__device__ __forceinline__ void input_at(const ConvArgs &p, const Span &sp, int64_t s, int64_t pos, int64_t c, pair_t (&r)[(V + 1) / 2]) {
     if (pos >= 0) {
-        const auto l = load_lump<io_t, V>(p.x, sp.row * p.x.sn + c * p.x.sc + (sp.start + pos) * p.x.st, 400);
-#pragma unroll
-        for (int i = 0; i < V; ++i) r[i] = l.v[i];
+        load_lump<io_t, V>(p.x, sp.row * p.x.sn + c * p.x.sc + (sp.start + pos) * p.x.st, 400).open(r);
     } else {
+        float f[V + 1] = {};
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            r[i] = p.state != nullptr ? load_one(static_cast<const io_t *>(p.state), (s * p.channels + c + i) * (W - 1) + W - 1 + pos,
-                                                 p.seq.count * p.channels * (W - 1), 401)
-                                      : 0.0f;
+            if (p.state != nullptr)
+                f[i] = load_one(static_cast<const io_t *>(p.state), (s * p.channels + c + i) * (W - 1) + W - 1 + pos,
+                                p.seq.count * p.channels * (W - 1), 401);
+#pragma unroll
+        for (int i = 0; i < (V + 1) / 2; ++i) r[i] = make_pair(f[2 * i], f[2 * i + 1]);
     }
 }
 
@@ -103,22 +138,36 @@ __device__ __forceinline__ void store_window(const ConvArgs &p, int64_t s, int64
     const Span sp = span_of(p.seq, s);
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
-        float r[V];
+        pair_t r[(V + 1) / 2];
         input_at<io_t, V, W>(p, sp, s, sp.length - (W - 1) + i, c, r);
 #pragma unroll
         for (int k = 0; k < V; ++k)
-            store_one(static_cast<io_t *>(p.state_out), (s * p.channels + c + k) * (W - 1) + i, p.seq.count * p.channels * (W - 1), 402, r[k]);
+            store_one(static_cast<io_t *>(p.state_out), (s * p.channels + c + k) * (W - 1) + i, p.seq.count * p.channels * (W - 1), 402,
+                      channel_of(r, k));
     }
 }
 
 template <typename io_t, int V, int W>
-__device__ __forceinline__ void load_taps(const ConvArgs &p, int64_t c, float (&w)[W][V], float (&bias)[V]) {
+__device__ __forceinline__ void load_taps(const ConvArgs &p, int64_t c, pair_t (&w)[W][(V + 1) / 2], pair_t (&bias)[(V + 1) / 2]) {
+    float f[W + 1][V + 1] = {};
 #pragma unroll
     for (int k = 0; k < V; ++k) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) w[i][k] = load_weight<io_t>(p.weight, p.weight_f32, (c + k) * W + i, p.channels * W, 403);
-        bias[k] = p.bias != nullptr ? load_weight<io_t>(p.bias, p.weight_f32, c + k, p.channels, 404) : 0.0f;
+        for (int i = 0; i < W; ++i) f[i][k] = load_weight<io_t>(p.weight, p.weight_f32, (c + k) * W + i, p.channels * W, 403);
+        if (p.bias != nullptr) f[W][k] = load_weight<io_t>(p.bias, p.weight_f32, c + k, p.channels, 404);
     }
+#pragma unroll
+    for (int k = 0; k < (V + 1) / 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) w[i][k] = make_pair(f[i][2 * k], f[i][2 * k + 1]);
+        bias[k] = make_pair(f[W][2 * k], f[W][2 * k + 1]);
+    }
+}
+
+__device__ __forceinline__ pair_t logistic2(pair_t v) {
+    const float2 x = halves(mul2(v, both(-kLog2e)));
+    const float2 d = halves(add2(make_pair(exp2_approx(x.x), exp2_approx(x.y)), both(1.0f)));
+    return make_pair(reciprocal_approx(d.x), reciprocal_approx(d.y));
 }
 
 // The flat grid's coordinates: channel blocks fastest, then blocks of chunks, then rows; the channels-last
@@ -132,7 +181,8 @@ __device__ __forceinline__ ConvBlock conv_block(const ConvArgs &p) {
 }
 
 template <typename io_t, int V, int W>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_cl_fwd_kernel(const __grid_constant__ ConvArgs p) {
+__global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_fwd_kernel(const __grid_constant__ ConvArgs p) {
+    constexpr int N = (V + 1) / 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const ConvBlock at = conv_block(p);
     const int64_t c = (at.channels * 32 + lane) * V;
@@ -149,7 +199,8 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_cl_fwd_kernel(const __gr
     if (t >= t_end) return;
     int64_t s = p.seq.offsets != nullptr ? find_sequence(p.seq, t, lane) : row;
     if (!live) return;
-    float w[W][V], bias[V];
+    const int64_t x0 = row * p.x.sn + c * p.x.sc, o0 = row * p.out.sn + c * p.out.sc;
+    pair_t w[W][N], bias[N];
     load_taps<io_t, V, W>(p, c, w, bias);
     Span sp = span_of(p.seq, s);
     while (t < t_end) {
@@ -163,38 +214,49 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_cl_fwd_kernel(const __gr
                 sp = span_of(p.seq, ++s);
                 continue;
             }
-            const float zero[V] = {};
-            for (; t < upto; ++t) store_lump<io_t, V>(p.out, row * p.out.sn + c * p.out.sc + t * p.out.st, 405, zero);
+            const pair_t zero[N] = {};
+            for (; t < upto; ++t) store_lump<io_t, V>(p.out, o0 + t * p.out.st, 405, zero);
             continue;
         }
+        constexpr int kAhead = 8;  // steps whose loads are in flight while the 8 before are worked on
         const int64_t end = sp.start + sp.length < t_end ? sp.start + sp.length : t_end;
-        float win[W - 1][V];
+        Lump<io_t, V> in[kAhead], next[kAhead];
+        const auto fetch = [&](int64_t from, Lump<io_t, V> (&to)[kAhead]) {
+            const int n = (int)(end - from);
+            int64_t at = x0 + from * p.x.st;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k, at += p.x.st)
+                if (k < n) to[k] = load_lump<io_t, V>(p.x, at, 400);
+        };
+        fetch(t, in);
+        pair_t win[W - 1][N];
 #pragma unroll
         for (int i = 0; i < W - 1; ++i) input_at<io_t, V, W>(p, sp, s, pos - (W - 1) + i, c, win[i]);
-        constexpr int kAhead = 8;  // loads in flight
         for (; t < end; t += kAhead) {
-            Lump<io_t, V> in[kAhead];
+            fetch(t + kAhead, next);
+            const int n = (int)(end - t);
+            int64_t to = o0 + t * p.out.st;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k)
-                if (t + k < end) in[k] = load_lump<io_t, V>(p.x, row * p.x.sn + c * p.x.sc + (t + k) * p.x.st, 400);
+            for (int k = 0; k < kAhead; ++k, to += p.out.st) {
+                if (k < n) {
+                    pair_t x[N], v[N];
+                    in[k].open(x);
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                if (t + k < end) {
-                    float v[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
+                    for (int i = 0; i < N; ++i) {
                         v[i] = bias[i];
 #pragma unroll
-                        for (int j = 0; j < W - 1; ++j) v[i] = fmaf(w[j][i], win[j][i], v[i]);
-                        v[i] = fmaf(w[W - 1][i], in[k].v[i], v[i]);
-                        if (p.silu) v[i] *= logistic(v[i]);
+                        for (int j = 0; j < W - 1; ++j) v[i] = fma2(w[j][i], win[j][i], v[i]);
+                        v[i] = fma2(w[W - 1][i], x[i], v[i]);
+                        if (p.silu) v[i] = mul2(v[i], logistic2(v[i]));
 #pragma unroll
                         for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-                        win[W - 2][i] = in[k].v[i];
+                        win[W - 2][i] = x[i];
                     }
-                    store_lump<io_t, V>(p.out, row * p.out.sn + c * p.out.sc + (t + k) * p.out.st, 405, v);
+                    store_lump<io_t, V>(p.out, to, 405, v);
                 }
             }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) in[k] = next[k];
         }
         t = end;
     }
@@ -219,8 +281,9 @@ __device__ __forceinline__ float carried_gradient(const ConvArgs &p, const ConvG
 // gv of step u + W-1 is known.  The sums over steps stay in registers, are added over the warps of
 // the CTA in shared memory and written as one part per CTA.
 template <typename io_t, int V, int W>
-__global__ void __launch_bounds__(kConvWarps * 32) conv_cl_bwd_kernel(const __grid_constant__ ConvArgs p,
-                                                                      const __grid_constant__ ConvGradArgs q) {
+__global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_bwd_kernel(const __grid_constant__ ConvArgs p,
+                                                                         const __grid_constant__ ConvGradArgs q) {
+    constexpr int N = (V + 1) / 2;
     __shared__ float sums[kConvWarps][(W + 1) * V][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const ConvBlock at = conv_block(p);
@@ -241,15 +304,16 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_cl_bwd_kernel(const __gr
     const int64_t row = at.row;
     int64_t t = (at.chunks * kConvWarps + warp) * kConvChunk;
     const int64_t t_end = t + kConvChunk < p.seq.steps ? t + kConvChunk : p.seq.steps;
-    float gw[W + 1][V];
+    pair_t gw[W + 1][N];
 #pragma unroll
     for (int i = 0; i <= W; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k) gw[i][k] = 0.0f;
+        for (int k = 0; k < N; ++k) gw[i][k] = 0;
     if (t < t_end) {
         int64_t s = p.seq.offsets != nullptr ? find_sequence(p.seq, t, lane) : row;
         if (live) {
-            float w[W][V], bias[V];
+            const int64_t x0 = row * p.x.sn + c * p.x.sc, g0 = row * q.gout.sn + c * q.gout.sc, o0 = row * q.gx.sn + c * q.gx.sc;
+            pair_t w[W][N], bias[N];
             load_taps<io_t, V, W>(p, c, w, bias);
             Span sp = span_of(p.seq, s);
             while (t < t_end) {
@@ -262,75 +326,98 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_cl_bwd_kernel(const __gr
                         sp = span_of(p.seq, ++s);
                         continue;
                     }
-                    const float zero[V] = {};
-                    for (; t < upto; ++t) store_lump<io_t, V>(q.gx, row * q.gx.sn + c * q.gx.sc + t * q.gx.st, 412, zero);
+                    const pair_t zero[N] = {};
+                    for (; t < upto; ++t) store_lump<io_t, V>(q.gx, o0 + t * q.gx.st, 412, zero);
                     continue;
                 }
+                constexpr int kAhead = 4;
                 const int64_t a = t, seq_end = sp.start + sp.length, b = seq_end < t_end ? seq_end : t_end;
-                float win[W - 1][V], part[W - 1][V];  // part[i]: gradient so far of the input W-1-i steps back
+                Lump<io_t, V> in[kAhead], up[kAhead], next_in[kAhead], next_up[kAhead];
+                const auto fetch = [&](int64_t from, Lump<io_t, V> (&x)[kAhead], Lump<io_t, V> (&g)[kAhead]) {
+                    const int n = (int)((b + W - 1 < seq_end ? b + W - 1 : seq_end) - from);
+                    int64_t at_x = x0 + from * p.x.st, at_g = g0 + from * q.gout.st;
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k, at_x += p.x.st, at_g += q.gout.st) {
+                        if (k < n) {
+                            x[k] = load_lump<io_t, V>(p.x, at_x, 400);
+                            g[k] = load_lump<io_t, V>(q.gout, at_g, 413);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < Lump<io_t, V>::kWords; ++i) x[k].w[i] = g[k].w[i] = 0;
+                        }
+                    }
+                };
+                fetch(t, in, up);
+                pair_t win[W - 1][N], part[W - 1][N];  // part[i]: gradient so far of the input W-1-i steps back
 #pragma unroll
                 for (int i = 0; i < W - 1; ++i) {
                     input_at<io_t, V, W>(p, sp, s, pos - (W - 1) + i, c, win[i]);
 #pragma unroll
-                    for (int k = 0; k < V; ++k) part[i][k] = 0.0f;
+                    for (int k = 0; k < N; ++k) part[i][k] = 0;
                 }
-                constexpr int kAhead = 4;
                 const int64_t last = b + W - 1;
                 for (; t < last; t += kAhead) {
-                    Lump<io_t, V> in[kAhead], up[kAhead];
+                    fetch(t + kAhead, next_in, next_up);
+                    const int n_last = (int)(last - t), n_b = (int)(b - t), n_seq = (int)(seq_end - t < kAhead ? seq_end - t : kAhead);
+                    int64_t to = o0 + (t - (W - 1)) * q.gx.st;
 #pragma unroll
-                    for (int k = 0; k < kAhead; ++k) {
-                        if (t + k < last && t + k < seq_end) {
-                            in[k] = load_lump<io_t, V>(p.x, row * p.x.sn + c * p.x.sc + (t + k) * p.x.st, 400);
-                            up[k] = load_lump<io_t, V>(q.gout, row * q.gout.sn + c * q.gout.sc + (t + k) * q.gout.st, 413);
-                        } else {
+                    for (int k = 0; k < kAhead; ++k, to += q.gx.st) {
+                        if (k < n_last) {
+                            pair_t x[N], g[N], done[N];
+                            in[k].open(x);
+                            up[k].open(g);
 #pragma unroll
-                            for (int i = 0; i < V; ++i) in[k].v[i] = up[k].v[i] = 0.0f;
-                        }
-                    }
+                            for (int i = 0; i < N; ++i) {
+                                pair_t gv = g[i];
+                                if (p.silu) {
+                                    pair_t v = bias[i];
 #pragma unroll
-                    for (int k = 0; k < kAhead; ++k) {
-                        const int64_t now = t + k;
-                        if (now < last) {
-                            float done[V];
-#pragma unroll
-                            for (int i = 0; i < V; ++i) {
-                                float v = bias[i];
-#pragma unroll
-                                for (int j = 0; j < W - 1; ++j) v = fmaf(w[j][i], win[j][i], v);
-                                v = fmaf(w[W - 1][i], in[k].v[i], v);
-                                const float gv = now < seq_end ? up[k].v[i] * activation_slope(v, p.silu) : 0.0f;
-                                if (now < b) {
-#pragma unroll
-                                    for (int j = 0; j < W - 1; ++j) gw[j][i] = fmaf(gv, win[j][i], gw[j][i]);
-                                    gw[W - 1][i] = fmaf(gv, in[k].v[i], gw[W - 1][i]);
-                                    gw[W][i] += gv;
+                                    for (int j = 0; j < W - 1; ++j) v = fma2(w[j][i], win[j][i], v);
+                                    v = fma2(w[W - 1][i], x[i], v);
+                                    const pair_t l = logistic2(v);
+                                    // silu'(v) = l (1 + v (1 - l))
+                                    gv = mul2(gv, mul2(l, fma2(v, fma2(l, both(-1.0f), both(1.0f)), both(1.0f))));
                                 }
-                                done[i] = fmaf(w[0][i], gv, part[0][i]);
+                                if (k >= n_seq) gv = 0;
+                                if (k < n_b) {
 #pragma unroll
-                                for (int j = 0; j + 1 < W - 1; ++j) part[j][i] = fmaf(w[j + 1][i], gv, part[j + 1][i]);
-                                part[W - 2][i] = w[W - 1][i] * gv;
+                                    for (int j = 0; j < W - 1; ++j) gw[j][i] = fma2(gv, win[j][i], gw[j][i]);
+                                    gw[W - 1][i] = fma2(gv, x[i], gw[W - 1][i]);
+                                    gw[W][i] = add2(gw[W][i], gv);
+                                }
+                                done[i] = fma2(w[0][i], gv, part[0][i]);
+#pragma unroll
+                                for (int j = 0; j + 1 < W - 1; ++j) part[j][i] = fma2(w[j + 1][i], gv, part[j + 1][i]);
+                                part[W - 2][i] = mul2(w[W - 1][i], gv);
 #pragma unroll
                                 for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-                                win[W - 2][i] = in[k].v[i];
+                                win[W - 2][i] = x[i];
                             }
-                            const int64_t u = now - (W - 1);  // the input whose gradient is complete
+                            const int64_t u = t + k - (W - 1);  // the input whose gradient is complete
                             if (u >= a || (a == sp.start && q.gstate != nullptr)) {
                                 const int64_t at_pos = u - sp.start;
-                                if (at_pos >= sp.length - (W - 1)) {
+                                if (q.gstate_out != nullptr && at_pos >= sp.length - (W - 1)) {
+                                    float f[V + 1] = {};
 #pragma unroll
-                                    for (int i = 0; i < V; ++i) done[i] += carried_gradient<io_t, W>(p, q, sp, s, at_pos, c + i);
+                                    for (int i = 0; i < V; ++i) f[i] = carried_gradient<io_t, W>(p, q, sp, s, at_pos, c + i);
+#pragma unroll
+                                    for (int i = 0; i < N; ++i) done[i] = add2(done[i], make_pair(f[2 * i], f[2 * i + 1]));
                                 }
                                 if (u >= a) {
-                                    store_lump<io_t, V>(q.gx, row * q.gx.sn + c * q.gx.sc + u * q.gx.st, 412, done);
+                                    store_lump<io_t, V>(q.gx, to, 412, done);
                                 } else {
 #pragma unroll
                                     for (int i = 0; i < V; ++i)
                                         store_one(static_cast<io_t *>(q.gstate), (s * p.channels + c + i) * (W - 1) + W - 1 + at_pos,
-                                                  p.seq.count * p.channels * (W - 1), 411, done[i]);
+                                                  p.seq.count * p.channels * (W - 1), 411, channel_of(done, i));
                                 }
                             }
                         }
+                    }
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) {
+                        in[k] = next_in[k];
+                        up[k] = next_up[k];
                     }
                 }
                 t = b;
@@ -340,7 +427,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_cl_bwd_kernel(const __gr
 #pragma unroll
     for (int i = 0; i <= W; ++i)
 #pragma unroll
-        for (int k = 0; k < V; ++k) sums[warp][i * V + k][lane] = gw[i][k];
+        for (int k = 0; k < V; ++k) sums[warp][i * V + k][lane] = channel_of(gw[i], k);
     __syncthreads();
     const int64_t part = at.row * p.chunk_blocks + at.chunks, parts = p.rows * p.chunk_blocks;
     for (int i = threadIdx.x; i < (W + 1) * V * 32; i += blockDim.x) {
@@ -369,24 +456,29 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_rows_fwd_kernel(const __
     const ConvBlock at = conv_block(p);
     const int64_t c = at.channels * kConvWarps + (threadIdx.x >> 5), row = at.row;
     if (c >= p.channels) return;
-    float w[W][1], bias[1];
-    load_taps<io_t, 1, W>(p, c, w, bias);
+    pair_t taps[W][1], bias[1];
+    load_taps<io_t, 1, W>(p, c, taps, bias);
+    const float b0 = halves(bias[0]).x;
+    float w[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = halves(taps[i][0]).x;
     const Span sp = span_of(p.seq, row);
     const int64_t x0 = row * p.x.sn + c * p.x.sc, o0 = row * p.out.sn + c * p.out.sc;
     for (int64_t t = (at.chunks * 32 + lane) * kRun; t < p.seq.steps; t += p.chunk_blocks * 32 * kRun) {
-        float in[kRun + W - 1], edge[1];
+        float in[kRun + W - 1];
+        pair_t edge[1];
         load_steps<io_t>(p.x, x0, t - (W - 1), 0, sp.length, 420, in);
 #pragma unroll
         for (int i = 0; i < W - 1; ++i)
             if (t - (W - 1) + i < 0) {
                 input_at<io_t, 1, W>(p, sp, row, t - (W - 1) + i, c, edge);
-                in[i] = edge[0];
+                in[i] = halves(edge[0]).x;
             }
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
-            float v = bias[0];
+            float v = b0;
 #pragma unroll
-            for (int j = 0; j < W; ++j) v = fmaf(w[j][0], in[k + j], v);
+            for (int j = 0; j < W; ++j) v = fmaf(w[j], in[k + j], v);
             if (p.silu) v *= logistic(v);
             if (t + k < p.seq.steps)
                 store_one(static_cast<io_t *>(p.out.data), o0 + (t + k) * p.out.st, p.out.extent, 421, t + k < sp.length ? v : 0.0f);
@@ -402,27 +494,32 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_rows_bwd_kernel(const __
     const ConvBlock at = conv_block(p);
     const int64_t c = at.channels * kConvWarps + (threadIdx.x >> 5), row = at.row;
     if (c >= p.channels) return;
-    float w[W][1], bias[1], gw[W + 1];
-    load_taps<io_t, 1, W>(p, c, w, bias);
+    pair_t taps[W][1], bias[1];
+    load_taps<io_t, 1, W>(p, c, taps, bias);
+    const float b0 = halves(bias[0]).x;
+    float w[W], gw[W + 1];
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = halves(taps[i][0]).x;
 #pragma unroll
     for (int i = 0; i <= W; ++i) gw[i] = 0.0f;
     const Span sp = span_of(p.seq, row);
     const int64_t x0 = row * p.x.sn + c * p.x.sc, g0 = row * q.gout.sn + c * q.gout.sc, o0 = row * q.gx.sn + c * q.gx.sc;
     for (int64_t t = (at.chunks * 32 + lane) * kRun; t < p.seq.steps; t += p.chunk_blocks * 32 * kRun) {
-        float in[kRun + 2 * (W - 1)], gv[kRun + W - 1], edge[1];
+        float in[kRun + 2 * (W - 1)], gv[kRun + W - 1];
+        pair_t edge[1];
         load_steps<io_t>(p.x, x0, t - (W - 1), 0, sp.length, 420, in);
         load_steps<io_t>(q.gout, g0, t, 0, sp.length, 422, gv);
 #pragma unroll
         for (int i = 0; i < W - 1; ++i)
             if (t - (W - 1) + i < 0) {
                 input_at<io_t, 1, W>(p, sp, row, t - (W - 1) + i, c, edge);
-                in[i] = edge[0];
+                in[i] = halves(edge[0]).x;
             }
 #pragma unroll
         for (int k = 0; k < kRun + W - 1; ++k) {
-            float v = bias[0];
+            float v = b0;
 #pragma unroll
-            for (int j = 0; j < W; ++j) v = fmaf(w[j][0], in[k + j], v);
+            for (int j = 0; j < W; ++j) v = fmaf(w[j], in[k + j], v);
             gv[k] = t + k < sp.length ? gv[k] * activation_slope(v, p.silu) : 0.0f;
             if (k < kRun) {
 #pragma unroll
@@ -434,7 +531,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_rows_bwd_kernel(const __
         for (int k = 0; k < kRun; ++k) {
             float v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < W; ++j) v = fmaf(w[j][0], gv[k + W - 1 - j], v);
+            for (int j = 0; j < W; ++j) v = fmaf(w[j], gv[k + W - 1 - j], v);
             if (t + k < sp.length) {
                 if (t + k >= sp.length - (W - 1)) v += carried_gradient<io_t, W>(p, q, sp, row, t + k, c);
             } else {
@@ -447,7 +544,7 @@ __global__ void __launch_bounds__(kConvWarps * 32) conv_rows_bwd_kernel(const __
             for (int i = 0; i < W - 1; ++i) {
                 float v = carried_gradient<io_t, W>(p, q, sp, row, i - (W - 1), c);
 #pragma unroll
-                for (int j = 0; j <= i; ++j) v = fmaf(w[j][0], gv[i - j], v);
+                for (int j = 0; j <= i; ++j) v = fmaf(w[j], gv[i - j], v);
                 store_one(static_cast<io_t *>(q.gstate), (row * p.channels + c) * (W - 1) + i, p.seq.count * p.channels * (W - 1), 411, v);
             }
         }
