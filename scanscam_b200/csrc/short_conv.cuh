@@ -15,7 +15,7 @@ namespace ssb {
 
 struct ConvArgs {
     int64_t channels, rows, channel_blocks, chunk_blocks;
-    int silu, weight_f32;
+    int silu, weight_f32, chunk;  // chunk: steps that a warp of the channels-last kernels walks
     Sequences seq;
     View3 x, out;
     const void *weight, *bias, *state;  // [C, W], [C]; [sequences, C, W-1] in the inputs' type
@@ -28,8 +28,10 @@ struct ConvGradArgs {
     float *part;  // [parts][C][W + 1]: gradients of the taps and the bias
 };
 
+struct True { static constexpr bool value = true; };
+struct False { static constexpr bool value = false; };
+
 constexpr int kConvWarps = 8;
-constexpr int kConvChunk = 32;  // steps a warp walks
 
 // The sequence that step t of a packed row lies in: the last one that starts at or before t (of
 // several that start there, the last is the one with steps).  The lanes look at 32 offsets at a time.
@@ -194,8 +196,8 @@ __global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_fwd_kernel(const _
         return;
     }
     const int64_t row = at.row;
-    int64_t t = (at.chunks * kConvWarps + warp) * kConvChunk;
-    const int64_t t_end = t + kConvChunk < p.seq.steps ? t + kConvChunk : p.seq.steps;
+    int64_t t = (at.chunks * kConvWarps + warp) * p.chunk;
+    const int64_t t_end = t + p.chunk < p.seq.steps ? t + p.chunk : p.seq.steps;
     if (t >= t_end) return;
     int64_t s = p.seq.offsets != nullptr ? find_sequence(p.seq, t, lane) : row;
     if (!live) return;
@@ -235,26 +237,30 @@ __global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_fwd_kernel(const _
         for (; t < end; t += kAhead) {
             fetch(t + kAhead, next);
             const int n = (int)(end - t);
-            int64_t to = o0 + t * p.out.st;
+            const auto group = [&](auto whole) {  // whole: all 8 steps exist, and nothing is asked per step
+                int64_t to = o0 + t * p.out.st;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k, to += p.out.st) {
-                if (k < n) {
-                    pair_t x[N], v[N];
-                    in[k].open(x);
+                for (int k = 0; k < kAhead; ++k, to += p.out.st) {
+                    if (decltype(whole)::value || k < n) {
+                        pair_t x[N], v[N];
+                        in[k].open(x);
 #pragma unroll
-                    for (int i = 0; i < N; ++i) {
-                        v[i] = bias[i];
+                        for (int i = 0; i < N; ++i) {
+                            v[i] = bias[i];
 #pragma unroll
-                        for (int j = 0; j < W - 1; ++j) v[i] = fma2(w[j][i], win[j][i], v[i]);
-                        v[i] = fma2(w[W - 1][i], x[i], v[i]);
-                        if (p.silu) v[i] = mul2(v[i], logistic2(v[i]));
+                            for (int j = 0; j < W - 1; ++j) v[i] = fma2(w[j][i], win[j][i], v[i]);
+                            v[i] = fma2(w[W - 1][i], x[i], v[i]);
+                            if (p.silu) v[i] = mul2(v[i], logistic2(v[i]));
 #pragma unroll
-                        for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-                        win[W - 2][i] = x[i];
+                            for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
+                            win[W - 2][i] = x[i];
+                        }
+                        store_lump<io_t, V>(p.out, to, 405, v);
                     }
-                    store_lump<io_t, V>(p.out, to, 405, v);
                 }
-            }
+            };
+            if (n >= kAhead) group(True{});
+            else group(False{});
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) in[k] = next[k];
         }
@@ -302,8 +308,8 @@ __global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_bwd_kernel(const _
         return;
     }
     const int64_t row = at.row;
-    int64_t t = (at.chunks * kConvWarps + warp) * kConvChunk;
-    const int64_t t_end = t + kConvChunk < p.seq.steps ? t + kConvChunk : p.seq.steps;
+    int64_t t = (at.chunks * kConvWarps + warp) * p.chunk;
+    const int64_t t_end = t + p.chunk < p.seq.steps ? t + p.chunk : p.seq.steps;
     pair_t gw[W + 1][N];
 #pragma unroll
     for (int i = 0; i <= W; ++i)
@@ -359,61 +365,69 @@ __global__ void __launch_bounds__(kConvWarps * 32, 2) conv_cl_bwd_kernel(const _
                 for (; t < last; t += kAhead) {
                     fetch(t + kAhead, next_in, next_up);
                     const int n_last = (int)(last - t), n_b = (int)(b - t), n_seq = (int)(seq_end - t < kAhead ? seq_end - t : kAhead);
-                    int64_t to = o0 + (t - (W - 1)) * q.gx.st;
+                    const bool inner = t - (W - 1) >= a && n_b >= kAhead && n_seq >= kAhead && q.gstate_out == nullptr;
+                    const auto group = [&](auto whole) {  // whole: the group lies inside the chunk, and nothing is asked per step
+                        constexpr bool kWhole = decltype(whole)::value;
+                        int64_t to = o0 + (t - (W - 1)) * q.gx.st;
 #pragma unroll
-                    for (int k = 0; k < kAhead; ++k, to += q.gx.st) {
-                        if (k < n_last) {
-                            pair_t x[N], g[N], done[N];
-                            in[k].open(x);
-                            up[k].open(g);
+                        for (int k = 0; k < kAhead; ++k, to += q.gx.st) {
+                            if (kWhole || k < n_last) {
+                                pair_t x[N], g[N], done[N];
+                                in[k].open(x);
+                                up[k].open(g);
 #pragma unroll
-                            for (int i = 0; i < N; ++i) {
-                                pair_t gv = g[i];
-                                if (p.silu) {
-                                    pair_t v = bias[i];
+                                for (int i = 0; i < N; ++i) {
+                                    pair_t gv = g[i];
+                                    if (p.silu) {
+                                        pair_t v = bias[i];
 #pragma unroll
-                                    for (int j = 0; j < W - 1; ++j) v = fma2(w[j][i], win[j][i], v);
-                                    v = fma2(w[W - 1][i], x[i], v);
-                                    const pair_t l = logistic2(v);
-                                    // silu'(v) = l (1 + v (1 - l))
-                                    gv = mul2(gv, mul2(l, fma2(v, fma2(l, both(-1.0f), both(1.0f)), both(1.0f))));
+                                        for (int j = 0; j < W - 1; ++j) v = fma2(w[j][i], win[j][i], v);
+                                        v = fma2(w[W - 1][i], x[i], v);
+                                        const pair_t l = logistic2(v);
+                                        // silu'(v) = l (1 + v (1 - l))
+                                        gv = mul2(gv, mul2(l, fma2(v, fma2(l, both(-1.0f), both(1.0f)), both(1.0f))));
+                                    }
+                                    if (!kWhole && k >= n_seq) gv = 0;
+                                    if (kWhole || k < n_b) {
+#pragma unroll
+                                        for (int j = 0; j < W - 1; ++j) gw[j][i] = fma2(gv, win[j][i], gw[j][i]);
+                                        gw[W - 1][i] = fma2(gv, x[i], gw[W - 1][i]);
+                                        gw[W][i] = add2(gw[W][i], gv);
+                                    }
+                                    done[i] = fma2(w[0][i], gv, part[0][i]);
+#pragma unroll
+                                    for (int j = 0; j + 1 < W - 1; ++j) part[j][i] = fma2(w[j + 1][i], gv, part[j + 1][i]);
+                                    part[W - 2][i] = mul2(w[W - 1][i], gv);
+#pragma unroll
+                                    for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
+                                    win[W - 2][i] = x[i];
                                 }
-                                if (k >= n_seq) gv = 0;
-                                if (k < n_b) {
-#pragma unroll
-                                    for (int j = 0; j < W - 1; ++j) gw[j][i] = fma2(gv, win[j][i], gw[j][i]);
-                                    gw[W - 1][i] = fma2(gv, x[i], gw[W - 1][i]);
-                                    gw[W][i] = add2(gw[W][i], gv);
-                                }
-                                done[i] = fma2(w[0][i], gv, part[0][i]);
-#pragma unroll
-                                for (int j = 0; j + 1 < W - 1; ++j) part[j][i] = fma2(w[j + 1][i], gv, part[j + 1][i]);
-                                part[W - 2][i] = mul2(w[W - 1][i], gv);
-#pragma unroll
-                                for (int j = 0; j + 1 < W - 1; ++j) win[j][i] = win[j + 1][i];
-                                win[W - 2][i] = x[i];
-                            }
-                            const int64_t u = t + k - (W - 1);  // the input whose gradient is complete
-                            if (u >= a || (a == sp.start && q.gstate != nullptr)) {
-                                const int64_t at_pos = u - sp.start;
-                                if (q.gstate_out != nullptr && at_pos >= sp.length - (W - 1)) {
-                                    float f[V + 1] = {};
-#pragma unroll
-                                    for (int i = 0; i < V; ++i) f[i] = carried_gradient<io_t, W>(p, q, sp, s, at_pos, c + i);
-#pragma unroll
-                                    for (int i = 0; i < N; ++i) done[i] = add2(done[i], make_pair(f[2 * i], f[2 * i + 1]));
-                                }
-                                if (u >= a) {
+                                const int64_t u = t + k - (W - 1);  // the input whose gradient is complete
+                                if (kWhole) {
                                     store_lump<io_t, V>(q.gx, to, 412, done);
-                                } else {
+                                } else if (u >= a || (a == sp.start && q.gstate != nullptr)) {
+                                    const int64_t at_pos = u - sp.start;
+                                    if (q.gstate_out != nullptr && at_pos >= sp.length - (W - 1)) {
+                                        float f[V + 1] = {};
 #pragma unroll
-                                    for (int i = 0; i < V; ++i)
-                                        store_one(static_cast<io_t *>(q.gstate), (s * p.channels + c + i) * (W - 1) + W - 1 + at_pos,
-                                                  p.seq.count * p.channels * (W - 1), 411, channel_of(done, i));
+                                        for (int i = 0; i < V; ++i) f[i] = carried_gradient<io_t, W>(p, q, sp, s, at_pos, c + i);
+#pragma unroll
+                                        for (int i = 0; i < N; ++i) done[i] = add2(done[i], make_pair(f[2 * i], f[2 * i + 1]));
+                                    }
+                                    if (u >= a) {
+                                        store_lump<io_t, V>(q.gx, to, 412, done);
+                                    } else {
+#pragma unroll
+                                        for (int i = 0; i < V; ++i)
+                                            store_one(static_cast<io_t *>(q.gstate), (s * p.channels + c + i) * (W - 1) + W - 1 + at_pos,
+                                                      p.seq.count * p.channels * (W - 1), 411, channel_of(done, i));
+                                    }
                                 }
                             }
                         }
-                    }
+                    };
+                    if (inner) group(True{});
+                    else group(False{});
 #pragma unroll
                     for (int k = 0; k < kAhead; ++k) {
                         in[k] = next_in[k];

@@ -47,89 +47,138 @@ __device__ __forceinline__ Turn turn_of(const Slots &s, int64_t m) {
 
 struct SelectiveStepArgs {
     int64_t channels, per_group, states;
-    int softplus, vec;  // vec: S is a multiple of 4 and the states and decays are 16-byte aligned
+    int softplus, vec, vec_proj;  // vec: S is a multiple of 4 and the states and decays are 16-byte aligned; vec_proj: 4 states of B and C likewise
     Slots slots;
     View2 x, dt, z, out, B, C;
     const float *A, *D, *dt_bias;
     float *state;
 };
 
+// N (a multiple of 4) adjacent elements, 8 (16-bit types) or 16 bytes at a time.
+template <typename T, int N>
+__device__ __forceinline__ void load_array(const T *p, int64_t at, int64_t extent, int site, float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        f[i] = f[i + 1] = f[i + 2] = f[i + 3] = 0.0f;
+        if (!SSB_VECTOR_OK(p + at + i, 4 * (int)sizeof(T), at + i + 3, extent, site)) continue;
+        if constexpr (sizeof(T) == 4) {
+            const float4 w = *reinterpret_cast<const float4 *>(p + at + i);
+            f[i] = w.x; f[i + 1] = w.y; f[i + 2] = w.z; f[i + 3] = w.w;
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2 *>(p + at + i);
+            unpack2<T>(w.x, f[i], f[i + 1]);
+            unpack2<T>(w.y, f[i + 2], f[i + 3]);
+        }
+    }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_array(T *p, int64_t at, int64_t extent, int site, const float (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        if (!SSB_VECTOR_OK(p + at + i, 4 * (int)sizeof(T), at + i + 3, extent, site)) continue;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        else *reinterpret_cast<uint2 *>(p + at + i) = make_uint2(pack2<T>(f[i], f[i + 1]), pack2<T>(f[i + 2], f[i + 3]));
+    }
+}
+
 // LANES lanes share a channel, each with 4 adjacent states at a time (one 16-byte access where S is
-// a multiple of 4); the read-out is summed over them by shuffles.
-template <typename io_t, int LANES>
+// a multiple of 4); the read-out is summed over them by shuffles.  A thread works on EACH channels, whose
+// states are on their way together: what has to be in flight is some 40 KB an SM.
+template <typename io_t, int LANES, int EACH>
 __global__ void __launch_bounds__(128) selective_step_kernel(const __grid_constant__ SelectiveStepArgs p) {
     constexpr int CB = 128 / LANES;
     const int64_t m0 = blockIdx.x;
     const int part = threadIdx.x % LANES;
-    const int64_t c = (int64_t)blockIdx.y * CB + threadIdx.x / LANES;
-    const bool live = c < p.channels;
+    const int64_t c0 = (int64_t)blockIdx.y * CB * EACH + threadIdx.x / LANES;
     const int S = (int)p.states;
     const Turn turn = turn_of(p.slots, m0);
     if (!turn.mine) return;
     if (turn.slot < 0) {
-        if (live && part == 0) store_one(static_cast<io_t *>(p.out.data), m0 * p.out.s0 + c * p.out.s1, p.out.extent, 300, 0.0f);
+#pragma unroll
+        for (int k = 0; k < EACH; ++k)
+            if (c0 + k * CB < p.channels && part == 0)
+                store_one(static_cast<io_t *>(p.out.data), m0 * p.out.s0 + (c0 + k * CB) * p.out.s1, p.out.extent, 300, 0.0f);
         return;
     }
-    const int64_t cc = live ? c : p.channels - 1;  // lanes behind the last channel stay for the shuffles
-    const int64_t g = cc / p.per_group;
-    const float D = p.D != nullptr ? load_one(p.D, cc, p.channels, 301) : 0.0f;
-    const float bias = p.dt_bias != nullptr ? load_one(p.dt_bias, cc, p.channels, 302) : 0.0f;
-    const bool vec = p.vec != 0;
     const int64_t state_extent = p.slots.pool * p.channels * S;
+    // 4 states of B or C; lanes behind the last channel stay for the shuffles, on the last channel's values
+    const auto projection = [&](const View2 &v, int64_t m, int64_t g, int n, int have, int site, float (&f)[4]) {
+        const int64_t at = m * v.s0 + g * v.s1 + n * v.s2;
+        if (p.vec_proj) {
+            load_array(static_cast<const io_t *>(v.data), at, v.extent, site, f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = i < have ? load_one(static_cast<const io_t *>(v.data), at + i * v.s2, v.extent, site) : 0.0f;
+        }
+    };
+    const auto quad = [&](const float *v, int64_t at, int have, int64_t extent, int site, float (&f)[4]) {
+        if (p.vec) {
+            load_array(v, at, extent, site, f);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = i < have ? load_one(v, at + i, extent, site) : 0.0f;
+        }
+    };
     for (int64_t m = m0; m < p.slots.entries; ++m) {
         if (m > m0) {
             if (!turn.more) break;
             if (p.slots.slots[m] != turn.slot) continue;
         }
-        const float x = load_one(static_cast<const io_t *>(p.x.data), m * p.x.s0 + cc * p.x.s1, p.x.extent, 303);
-        float dt = load_one(static_cast<const io_t *>(p.dt.data), m * p.dt.s0 + cc * p.dt.s1, p.dt.extent, 304) + bias;
-        if (p.softplus) dt = softplus(dt);
-        const float u = dt * x;
-        float y = 0.0f;
+        float x[EACH], dt[EACH], y[EACH], z[EACH];
+        int64_t cc[EACH];
+#pragma unroll
+        for (int k = 0; k < EACH; ++k) {
+            cc[k] = c0 + k * CB < p.channels ? c0 + k * CB : p.channels - 1;
+            x[k] = load_one(static_cast<const io_t *>(p.x.data), m * p.x.s0 + cc[k] * p.x.s1, p.x.extent, 303);
+            dt[k] = load_one(static_cast<const io_t *>(p.dt.data), m * p.dt.s0 + cc[k] * p.dt.s1, p.dt.extent, 304);
+            if (p.dt_bias != nullptr) dt[k] += load_one(p.dt_bias, cc[k], p.channels, 302);
+            z[k] = p.z.data != nullptr ? load_one(static_cast<const io_t *>(p.z.data), m * p.z.s0 + cc[k] * p.z.s1, p.z.extent, 310) : 0.0f;
+            y[k] = 0.0f;
+        }
         for (int n = part * 4; n < S; n += LANES * 4) {
-            const int64_t at = (turn.slot * p.channels + cc) * S + n;
             const int have = S - n < 4 ? S - n : 4;
-            float h[4] = {0, 0, 0, 0}, a[4] = {0, 0, 0, 0};
-            if (vec && SSB_VECTOR_OK(p.state + at, 16, at + 3, state_extent, 305) && SSB_VECTOR_OK(p.A + cc * S + n, 16, cc * S + n + 3, p.channels * S, 306)) {
-                const float4 hv = *reinterpret_cast<const float4 *>(p.state + at);
-                const float4 av = *reinterpret_cast<const float4 *>(p.A + cc * S + n);
-                h[0] = hv.x; h[1] = hv.y; h[2] = hv.z; h[3] = hv.w;
-                a[0] = av.x; a[1] = av.y; a[2] = av.z; a[3] = av.w;
-            } else {
+            float h[EACH][4], a[EACH][4], b[4], r[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (i < have) {
-                        h[i] = load_one(p.state, at + i, state_extent, 305);
-                        a[i] = load_one(p.A, cc * S + n + i, p.channels * S, 306);
-                    }
+            for (int k = 0; k < EACH; ++k) {
+                quad(p.state, (turn.slot * p.channels + cc[k]) * S + n, have, state_extent, 305, h[k]);
+                quad(p.A, cc[k] * S + n, have, p.channels * S, 306, a[k]);
             }
+            int64_t group = -1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (i < have) {
-                    const float b = load_one(static_cast<const io_t *>(p.B.data), m * p.B.s0 + g * p.B.s1 + (n + i) * p.B.s2, p.B.extent, 307);
-                    const float r = load_one(static_cast<const io_t *>(p.C.data), m * p.C.s0 + g * p.C.s1 + (n + i) * p.C.s2, p.C.extent, 308);
-                    h[i] = fmaf(exp2_approx(dt * (a[i] * kLog2e)), h[i], u * b);
-                    y = fmaf(r, h[i], y);
+            for (int k = 0; k < EACH; ++k) {
+                const int64_t g = p.per_group == p.channels ? 0 : cc[k] / p.per_group;
+                if (g != group) {
+                    projection(p.B, m, g, n, have, 307, b);
+                    projection(p.C, m, g, n, have, 308, r);
+                    group = g;
                 }
-            if (live) {
-                if (vec && SSB_VECTOR_OK(p.state + at, 16, at + 3, state_extent, 309)) {
-                    *reinterpret_cast<float4 *>(p.state + at) = make_float4(h[0], h[1], h[2], h[3]);
-                } else {
+                const float d = n == part * 4 ? (dt[k] = p.softplus ? softplus(dt[k]) : dt[k]) : dt[k], u = d * x[k];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (i < have) store_one(p.state, at + i, state_extent, 309, h[i]);
+                for (int i = 0; i < 4; ++i) {
+                    h[k][i] = fmaf(exp2_approx(d * (a[k][i] * kLog2e)), h[k][i], u * b[i]);
+                    if (i < have) y[k] = fmaf(r[i], h[k][i], y[k]);
+                }
+                if (c0 + k * CB < p.channels) {
+                    const int64_t at = (turn.slot * p.channels + cc[k]) * S + n;
+                    if (p.vec) {
+                        store_array(p.state, at, state_extent, 309, h[k]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (i < have) store_one(p.state, at + i, state_extent, 309, h[k][i]);
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int d = LANES / 2; d >= 1; d >>= 1) y += __shfl_xor_sync(kFullMask, y, d);
-        if (live && part == 0) {
-            y = fmaf(D, x, y);
-            if (p.z.data != nullptr) {
-                const float z = load_one(static_cast<const io_t *>(p.z.data), m * p.z.s0 + cc * p.z.s1, p.z.extent, 310);
-                y *= z * logistic(z);
+        for (int k = 0; k < EACH; ++k) {
+#pragma unroll
+            for (int d = LANES / 2; d >= 1; d >>= 1) y[k] += __shfl_xor_sync(kFullMask, y[k], d);
+            if (c0 + k * CB < p.channels && part == 0) {
+                if (p.D != nullptr) y[k] = fmaf(load_one(p.D, cc[k], p.channels, 301), x[k], y[k]);
+                if (p.z.data != nullptr) y[k] *= z[k] * logistic(z[k]);
+                store_one(static_cast<io_t *>(p.out.data), m * p.out.s0 + cc[k] * p.out.s1, p.out.extent, 300, y[k]);
             }
-            store_one(static_cast<io_t *>(p.out.data), m * p.out.s0 + c * p.out.s1, p.out.extent, 300, y);
         }
     }
 }
@@ -148,42 +197,70 @@ __device__ __forceinline__ float load_weight(const void *w, int f32, int64_t at,
     return f32 ? load_one(static_cast<const float *>(w), at, extent, site) : load_one(static_cast<const io_t *>(w), at, extent, site);
 }
 
-template <typename io_t, int W>
+// V adjacent channels a thread: 4 where their pieces are whole and aligned, else 1.
+template <typename io_t, int W, int V>
 __global__ void __launch_bounds__(128) conv_step_kernel(const __grid_constant__ ConvStepArgs p) {
-    const int64_t m0 = blockIdx.x, c = (int64_t)blockIdx.y * 128 + threadIdx.x;
+    const int64_t m0 = blockIdx.x, c = ((int64_t)blockIdx.y * 128 + threadIdx.x) * V;
     const Turn turn = turn_of(p.slots, m0);
     if (!turn.mine || c >= p.channels) return;
     io_t *out = static_cast<io_t *>(p.out.data);
+    const auto put = [&](int64_t m, const float (&v)[V]) {
+        const int64_t at = m * p.out.s0 + c * p.out.s1;
+        if constexpr (V == 4) store_array(out, at, p.out.extent, 320, v);
+        else store_one(out, at, p.out.extent, 320, v[0]);
+    };
     if (turn.slot < 0) {
-        store_one(out, m0 * p.out.s0 + c * p.out.s1, p.out.extent, 320, 0.0f);
+        const float zero[V] = {};
+        put(m0, zero);
         return;
     }
     io_t *state = static_cast<io_t *>(p.state);
     const int64_t at = (turn.slot * p.channels + c) * (W - 1), extent = p.slots.pool * p.channels * (W - 1);
-    float w[W], seen[W - 1];
+    float w[V * W], bias[V] = {}, seen[V * (W - 1)];  // [channel][tap], [channel][input]
+    if constexpr (V == 4) {
+        load_array(state, at, extent, 323, seen);
+        if (p.weight_f32) {
+            load_array(static_cast<const float *>(p.weight), c * W, p.channels * W, 321, w);
+            if (p.bias != nullptr) load_array(static_cast<const float *>(p.bias), c, p.channels, 322, bias);
+        } else {
+            load_array(static_cast<const io_t *>(p.weight), c * W, p.channels * W, 321, w);
+            if (p.bias != nullptr) load_array(static_cast<const io_t *>(p.bias), c, p.channels, 322, bias);
+        }
+    } else {
 #pragma unroll
-    for (int i = 0; i < W; ++i) w[i] = load_weight<io_t>(p.weight, p.weight_f32, c * W + i, p.channels * W, 321);
-    const float bias = p.bias != nullptr ? load_weight<io_t>(p.bias, p.weight_f32, c, p.channels, 322) : 0.0f;
+        for (int i = 0; i < W - 1; ++i) seen[i] = load_one(state, at + i, extent, 323);
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) seen[i] = load_one(state, at + i, extent, 323);
+        for (int i = 0; i < W; ++i) w[i] = load_weight<io_t>(p.weight, p.weight_f32, c * W + i, p.channels * W, 321);
+        if (p.bias != nullptr) bias[0] = load_weight<io_t>(p.bias, p.weight_f32, c, p.channels, 322);
+    }
     for (int64_t m = m0; m < p.slots.entries; ++m) {
         if (m > m0) {
             if (!turn.more) break;
             if (p.slots.slots[m] != turn.slot) continue;
         }
-        const float x = load_one(static_cast<const io_t *>(p.x.data), m * p.x.s0 + c * p.x.s1, p.x.extent, 324);
-        float v = bias;
+        float x[V], v[V];
+        const int64_t from = m * p.x.s0 + c * p.x.s1;
+        if constexpr (V == 4) load_array(static_cast<const io_t *>(p.x.data), from, p.x.extent, 324, x);
+        else x[0] = load_one(static_cast<const io_t *>(p.x.data), from, p.x.extent, 324);
 #pragma unroll
-        for (int i = 0; i < W - 1; ++i) v = fmaf(w[i], seen[i], v);
-        v = fmaf(w[W - 1], x, v);
-        if (p.silu) v *= logistic(v);
-        store_one(out, m * p.out.s0 + c * p.out.s1, p.out.extent, 320, v);
+        for (int k = 0; k < V; ++k) {
+            v[k] = bias[k];
 #pragma unroll
-        for (int i = 0; i + 1 < W - 1; ++i) seen[i] = seen[i + 1];
-        seen[W - 2] = x;
+            for (int i = 0; i < W - 1; ++i) v[k] = fmaf(w[k * W + i], seen[k * (W - 1) + i], v[k]);
+            v[k] = fmaf(w[k * W + W - 1], x[k], v[k]);
+            if (p.silu) v[k] *= logistic(v[k]);
+#pragma unroll
+            for (int i = 0; i + 1 < W - 1; ++i) seen[k * (W - 1) + i] = seen[k * (W - 1) + i + 1];
+            seen[k * (W - 1) + W - 2] = x[k];
+        }
+        put(m, v);
     }
+    if constexpr (V == 4) {
+        store_array(state, at, extent, 323, seen);
+    } else {
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) store_one(state, at + i, extent, 323, seen[i]);
+        for (int i = 0; i < W - 1; ++i) store_one(state, at + i, extent, 323, seen[i]);
+    }
 }
 
 }  // namespace ssb

@@ -311,6 +311,14 @@ struct ConvForm {
 bool lumps(const ssb_view_t &v, int dtype) {
     return v.stride[1] == 1 && v.stride[0] % 4 == 0 && v.stride[2] % 4 == 0 && aligned(v.data, 4 * size_of(dtype));
 }
+// Steps a warp walks: the more, the fewer steps are read twice (W - 1 a chunk) and the shorter the chunk's ends weigh
+// ([8, 4096, 2048], bf16: 73 and 141 us forward and backward with 64 steps, 80 and 167 with 32), but the SMs want
+// three CTAs each.
+int conv_chunk(const ssb_short_conv_t *p) {
+    for (int chunk = 64; chunk > 16; chunk /= 2)
+        if ((p->channels + 127) / 128 * p->batch * ((p->steps + ssb::kConvWarps * chunk - 1) / (ssb::kConvWarps * chunk)) >= 3 * sm_count()) return chunk;
+    return 16;
+}
 ConvForm conv_form(const ssb_short_conv_t *p, std::initializer_list<const ssb_view_t *> views) {
     bool cl = true, vec = p->channels % 4 == 0;
     for (const ssb_view_t *v : views) {
@@ -319,14 +327,14 @@ ConvForm conv_form(const ssb_short_conv_t *p, std::initializer_list<const ssb_vi
     }
     // time adjacent as well (one channel, or one step): the rows kernels do as well, but packed rows need the others
     ConvForm f{cl, vec ? 4 : 1, 0, 0};
-    const int64_t chunk = cl ? ssb::kConvChunk * ssb::kConvWarps : 4 * 32 * ssb::kRun;
+    const int64_t chunk = cl ? conv_chunk(p) * ssb::kConvWarps : 4 * 32 * ssb::kRun;
     f.channel_blocks = cl ? (p->channels + 32 * f.lump - 1) / (32 * f.lump) : (p->channels + ssb::kConvWarps - 1) / ssb::kConvWarps;
     f.chunk_blocks = std::max<int64_t>(1, (p->steps + chunk - 1) / chunk);
     return f;
 }
 // Parts of the taps' gradient: the same for either form and lump, so that the query needs no views.
 int64_t conv_parts(const ssb_short_conv_t *p) {
-    const int64_t chunk = ssb::kConvChunk * ssb::kConvWarps;
+    const int64_t chunk = conv_chunk(p) * ssb::kConvWarps;  // 512 at most; the rows form has chunks of 1024
     return std::max<int64_t>(1, p->batch) * std::max<int64_t>(1, (p->steps + chunk - 1) / chunk);
 }
 
@@ -338,6 +346,7 @@ ssb::ConvArgs conv_args(const ssb_short_conv_t *p, const ConvForm &f) {
     a.chunk_blocks = f.chunk_blocks;
     a.silu = p->silu;
     a.weight_f32 = p->weight_f32;
+    a.chunk = conv_chunk(p);
     a.seq = sequences_of(p->batch, p->steps, p->sequences, p->offsets, p->lengths);
     a.x = view3(p->x, p->dtype, p->batch, p->channels, p->steps, false, false);
     a.out = view3(p->out, p->dtype, p->batch, p->channels, p->steps, false, false);
@@ -537,6 +546,9 @@ int ssb_selective_step(const ssb_selective_step_t *p, void *stream) {
     a.states = p->states;
     a.softplus = p->softplus;
     a.vec = p->states % 4 == 0 && aligned(p->state, 16) && aligned(p->A, 16);
+    a.vec_proj = p->states % 4 == 0;
+    for (const ssb_view_t *v : {&p->B, &p->C})
+        a.vec_proj = a.vec_proj && aligned(v->data, 4 * size_of(p->dtype)) && v->stride[2] == 1 && v->stride[0] % 4 == 0 && v->stride[1] % 4 == 0;
     a.slots = {p->slots, p->entries, p->pool};
     a.x = view2(p->x, p->entries, p->channels);
     a.dt = view2(p->dt, p->entries, p->channels);
@@ -550,17 +562,23 @@ int ssb_selective_step(const ssb_selective_step_t *p, void *stream) {
     a.state = p->state;
     return with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
-        const auto launch = [&](auto kernel, int lanes) {
-            const int64_t blocks = (p->channels + 128 / lanes - 1) / (128 / lanes);
+        // 4 channels a thread, their loads under way together, where that leaves the SMs two CTAs each
+        const auto launch = [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value, CB = 128 / L;
+            const bool many = p->entries * ((p->channels + 4 * CB - 1) / (4 * CB)) >= 2 * sm_count();
+            const int64_t blocks = (p->channels + CB * (many ? 4 : 1) - 1) / (CB * (many ? 4 : 1));
             if (blocks > 65535) return fail(SSB_ERR_UNSUPPORTED, "too many channels");
-            kernel<<<dim3((unsigned)p->entries, (unsigned)blocks), 128, 0, (cudaStream_t)stream>>>(a);
+            const dim3 grid((unsigned)p->entries, (unsigned)blocks);
+            if (many) ssb::selective_step_kernel<io_t, L, 4><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
+            else ssb::selective_step_kernel<io_t, L, 1><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
             return check_launch("selective_step_kernel");
         };
-        if (p->states <= 4) return launch(ssb::selective_step_kernel<io_t, 1>, 1);
-        if (p->states <= 8) return launch(ssb::selective_step_kernel<io_t, 2>, 2);
-        if (p->states <= 16) return launch(ssb::selective_step_kernel<io_t, 4>, 4);
-        if (p->states <= 32) return launch(ssb::selective_step_kernel<io_t, 8>, 8);
-        return launch(ssb::selective_step_kernel<io_t, 16>, 16);
+        using std::integral_constant;
+        if (p->states <= 4) return launch(integral_constant<int, 1>{});
+        if (p->states <= 8) return launch(integral_constant<int, 2>{});
+        if (p->states <= 16) return launch(integral_constant<int, 4>{});
+        if (p->states <= 32) return launch(integral_constant<int, 8>{});
+        return launch(integral_constant<int, 16>{});
     });
 }
 
@@ -669,9 +687,16 @@ int ssb_short_conv_step(const ssb_short_conv_step_t *p, void *stream) {
         using io_t = std::remove_pointer_t<decltype(type)>;
         return with_width(p->width, [&](auto k) {
             constexpr int W = decltype(k)::value;
-            const int64_t blocks = (p->channels + 127) / 128;
+            // 4 channels a thread where all their pieces are whole and aligned
+            const size_t piece = 4 * size_of(p->dtype), wide = 4 * (p->weight_f32 ? 4 : size_of(p->dtype));
+            const bool lumps = p->channels % 4 == 0 && aligned(p->state, piece) && aligned(p->weight, wide) && aligned(p->bias, wide) &&
+                               aligned(p->x.data, piece) && p->x.stride[1] == 1 && p->x.stride[0] % 4 == 0 &&
+                               aligned(p->out.data, piece) && p->out.stride[1] == 1 && p->out.stride[0] % 4 == 0;
+            const int64_t blocks = (p->channels + 128 * (lumps ? 4 : 1) - 1) / (128 * (lumps ? 4 : 1));
             if (blocks > 65535) return fail(SSB_ERR_UNSUPPORTED, "too many channels");
-            ssb::conv_step_kernel<io_t, W><<<dim3((unsigned)p->entries, (unsigned)blocks), 128, 0, (cudaStream_t)stream>>>(a);
+            const dim3 grid((unsigned)p->entries, (unsigned)blocks);
+            if (lumps) ssb::conv_step_kernel<io_t, W, 4><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
+            else ssb::conv_step_kernel<io_t, W, 1><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
             return check_launch("conv_step_kernel");
         });
     });

@@ -137,6 +137,74 @@ def test_scan_with_many_channels(n, c, t):
     check_scan(o, True, ref.spans_of(n, t))
 
 
+# The forms that are chosen where channels and sequences abound: 8 states a lane in the forward (from 37 888 channels
+# x sequences x eighths of the states up), lanes across states in the backward (from 18 944 x quarters, up to 32 states).
+MANY = [("rows", F32, 10, 520, 33, 16, 2), ("cl", BF16, 10, 520, 70, 16, 1), ("slice", F16, 5, 1000, 40, 13, 1), ("cl", F32, 6, 800, 31, 16, 1),
+        ("strided", BF16, 10, 501, 20, 16, 1), ("cl", BF16, 3, 802, 48, 32, 2), ("cl", F32, 12, 800, 17, 7, 1), ("rows", BF16, 40, 512, 64, 16, 1),
+        ("cl", F16, 38, 513, 9, 16, 3), ("cl", BF16, 20, 500, 12, 32, 1), ("cl", F32, 5, 1000, 1, 16, 1), ("rows", F16, 12, 808, 40, 8, 1)]
+
+
+@pytest.mark.parametrize("layout,dtype,n,c,t,s,g", MANY, ids=str)
+def test_scan_with_many_channels_and_sequences(layout, dtype, n, c, t, s, g):
+    o = make_scan(dtype, layout, n, c, t, s, g, state=True, seed=n + s)
+    check_scan(o, True, ref.spans_of(n, t))
+
+
+@pytest.mark.parametrize("missing", ["D", "z", "bias", "softplus", "all"])
+def test_scan_with_many_channels_without_optional_operands(missing):
+    names = ("D", "z", "bias", "softplus") if missing == "all" else (missing,)
+    have = {k: k not in names for k in ("D", "z", "bias", "softplus")}
+    o = make_scan(F32, "cl", 10, 500, 35, 16, seed=23, **have)
+    check_scan(o, have["softplus"], ref.spans_of(10, 35))
+
+
+@pytest.mark.parametrize("dtype,layout", [(F32, "cl"), (BF16, "cl"), (F16, "rows")])
+def test_scan_packed_with_many_sequences(dtype, layout):
+    """Empty ones, single steps, bounds at and off the runs of 16 and the tiles of 32 steps; steps that belong to none."""
+    offsets = [2, 2, 3, 19, 35, 35, 67, 99, 100, 116, 133, 133, 150, 151, 152, 168, 200, 231, 264, 264, 265, 281, 290, 291, 300]
+    t, count = 303, len(offsets) - 1
+    o = make_scan(dtype, layout, 1, 212, t, 16, 2, state=True, count=count, seed=24)
+    clean = {k: v.clone() for k, v in o.items()}
+    for k in ("x", "dt", "z", "B", "C"):
+        o[k] = o[k].clone()
+        o[k][..., : offsets[0]] = NAN
+        o[k][..., offsets[-1]:] = INF
+    got, gout, gstate = run_scan(o, True, offsets=ints(offsets))
+    want = ref.scan_selective(**clean, dt_softplus=True, spans=ref.spans_of(1, t, offsets=offsets), gout=gout, gstate=gstate)
+    base, channels, steps = scan_roundings(clean, True)
+    for k, v in got.items():
+        ref.check(v, want[k], dtype if k in ("out", "gx", "gdt", "gz", "gB", "gC") else F32, base + channels + steps, k)
+
+
+def test_scan_padded_batch_of_many_channels():
+    lengths, t = [0, 1, 16, 17, 32, 33, 40, 47, 48, 50], 50
+    o = make_scan(F32, "cl", 10, 500, t, 16, state=True, seed=25)
+    clean = {k: v.clone() for k, v in o.items()}
+    for k in ("x", "dt", "z", "B", "C"):
+        o[k] = o[k].clone()
+        for i, size in enumerate(lengths):
+            o[k][i, ..., size:] = NAN if i % 2 else -INF
+    got, gout, gstate = run_scan(o, True, lengths=ints(lengths))
+    want = ref.scan_selective(**clean, dt_softplus=True, spans=ref.spans_of(10, t, lengths), gout=gout, gstate=gstate)
+    base, channels, steps = scan_roundings(clean, True)
+    for k, v in got.items():
+        ref.check(v, want[k], F32, base + channels + steps, k)
+
+
+def test_scan_of_many_channels_is_repeatable():
+    o = make_scan(BF16, "cl", 10, 520, 150, 16, seed=26)
+    first, _, _ = run_scan(o, True)
+    for _ in range(3):
+        again, _, _ = run_scan(o, True)
+        assert all(torch.equal(first[k], again[k]) for k in first)
+
+
+def test_scan_more_sequences_than_a_block_of_sums():
+    """The CTAs of the backward take several sequences each."""
+    o = make_scan(F32, "cl", 90, 260, 18, 16, state=True, seed=27)
+    check_scan(o, True, ref.spans_of(90, 18))
+
+
 @pytest.mark.parametrize("dtype,layout", [(F32, "cl"), (BF16, "cl"), (F32, "rows"), (F16, "rows")])
 @pytest.mark.parametrize("offsets,t", [([0, 5, 5, 6, 70, 70, 135], 135), ([3, 3, 40, 41, 110], 120), ([0, 0], 9), ([0, 64, 128, 192], 192), ([7, 7, 7], 20)])
 def test_scan_packed(dtype, layout, offsets, t):
@@ -354,7 +422,7 @@ def check_conv(o, silu, spans, back="both", clean=None, **more):
 
 
 @pytest.mark.parametrize("n,c,t,w", [(1, 1, 1, 4), (2, 3, 2, 3), (1, 4, 3, 4), (3, 36, 8, 2), (1, 130, 31, 4), (2, 64, 33, 3), (1, 12, 255, 4),
-                                     (2, 515, 65, 4), (1, 8, 1030, 3), (1, 260, 300, 2)])
+                                     (2, 515, 65, 4), (1, 8, 1030, 3), (1, 260, 300, 2), (7, 2052, 600, 4), (60, 1028, 40, 3)])
 @pytest.mark.parametrize("dtype,layout", [(F32, "rows"), (BF16, "cl"), (F16, "slice"), (F32, "strided"), (F32, "cl"), (BF16, "rows")])
 def test_conv_and_gradients(n, c, t, w, dtype, layout):
     check_conv(make_conv(dtype, layout, n, c, t, w, state=t % 2 == 1, bias=c != 64, seed=n + c + t), t != 31, ref.spans_of(n, t))
@@ -447,7 +515,8 @@ def step_reference(x, dt, A, B, C, state, D, z, bias, softplus, slots):
 @pytest.mark.parametrize("m,c,s,g,pool,slots", [
     (1, 1, 1, 1, 1, None), (1, 2048, 16, 1, 1, None), (3, 33, 7, 3, 3, None), (5, 64, 16, 2, 9, [8, -1, 0, 3, 9]), (4, 40, 64, 1, 6, [2, 2, 2, 2]),
     (6, 17, 256, 1, 4, [0, 3, 0, -5, 3, 1]), (2, 10, 33, 5, 2, [1, 0]), (300, 20, 4, 1, 40, [i * 7 % 43 for i in range(300)]), (0, 8, 4, 1, 3, []),
-    (2, 8, 4, 1, 0, [0, -1])])
+    (2, 8, 4, 1, 0, [0, -1]), (40, 1001, 16, 1, 40, None), (64, 520, 16, 2, 70, [(i * 11) % 71 - 1 for i in range(64)]), (300, 66, 64, 3, 300, None),
+    (300, 130, 13, 1, 40, [i * 7 % 43 for i in range(300)])])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_scan_step(m, c, s, g, pool, slots, dtype):
     o = {"x": randn(m, c, seed=1, dtype=dtype), "dt": randn(m, 2 * c, seed=2, dtype=dtype)[:, c:], "A": -torch.exp(randn(c, s, seed=3)),
