@@ -62,6 +62,24 @@ __device__ __forceinline__ pair_t shfl_down2(pair_t p, int delta) {
     return make_pair(__shfl_down_sync(kFullMask, f.x, delta), __shfl_down_sync(kFullMask, f.y, delta));
 }
 
+// Sums v[i] over LN neighbouring lanes; lane q of them is left with the sum of v[q mod STEPS].
+template <int LN, int STEPS>
+__device__ __forceinline__ float sum_and_spread(float (&v)[STEPS], int q) {
+    static_assert(STEPS <= LN, "a lane is left with one sum");
+#pragma unroll
+    for (int half = STEPS / 2; half >= 1; half >>= 1) {
+        const bool upper = (q & half) != 0;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+            const float give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
+            v[i] = keep + __shfl_xor_sync(kFullMask, give, half);
+        }
+    }
+#pragma unroll
+    for (int d = STEPS; d < LN; d <<= 1) v[0] += __shfl_xor_sync(kFullMask, v[0], d);
+    return v[0];
+}
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -169,24 +169,6 @@ struct ProjectionPieces {
     }
 };
 
-// Sums v[i] of step i over the LN lanes of a channel; lane q of them is left with the sum of step q mod STEPS.
-template <int LN, int STEPS>
-__device__ __forceinline__ float sum_and_spread(float (&v)[STEPS], int q) {
-    static_assert(STEPS <= LN, "a lane is left with one step");
-#pragma unroll
-    for (int half = STEPS / 2; half >= 1; half >>= 1) {
-        const bool upper = (q & half) != 0;
-#pragma unroll
-        for (int i = 0; i < half; ++i) {
-            const float give = upper ? v[i] : v[i + half], keep = upper ? v[i + half] : v[i];
-            v[i] = keep + __shfl_xor_sync(kFullMask, give, half);
-        }
-    }
-#pragma unroll
-    for (int d = STEPS; d < LN; d <<= 1) v[0] += __shfl_xor_sync(kFullMask, v[0], d);
-    return v[0];
-}
-
 template <int LN, int SPL, int WARPS>
 struct LaneShape {
     static constexpr int SP = LN * SPL;                  // states, padded

@@ -82,28 +82,32 @@ __device__ __forceinline__ void store_array(T *p, int64_t at, int64_t extent, in
 }
 
 // LANES lanes share a channel, each with 4 adjacent states at a time (one 16-byte access where S is
-// a multiple of 4); the read-out is summed over them by shuffles.  A thread works on EACH channels, whose
-// states are on their way together: what has to be in flight is some 40 KB an SM.
+// a multiple of 4).  EACH adjacent channels a thread, 4 or 1: with 4, each lane of a quad prepares one of the
+// four channels (its step size, input, gate) and hands it to the others, and the sums over the states are
+// exchanged so that each is left with one.  Instructions bound the large calls, not the states' bytes: with every
+// lane preparing every channel, 256 entries of 4096 channels took 59 us whatever the loads in flight.
 template <typename io_t, int LANES, int EACH>
 __global__ void __launch_bounds__(128) selective_step_kernel(const __grid_constant__ SelectiveStepArgs p) {
-    constexpr int CB = 128 / LANES;
+    static_assert(EACH == 1 || (EACH == 4 && LANES >= 4), "a lane of a quad for each channel");
+    constexpr int CB = 128 / LANES * EACH;
     const int64_t m0 = blockIdx.x;
     const int part = threadIdx.x % LANES;
-    const int64_t c0 = (int64_t)blockIdx.y * CB * EACH + threadIdx.x / LANES;
+    const int64_t first = (int64_t)blockIdx.y * CB + threadIdx.x / LANES * EACH;
     const int S = (int)p.states;
     const Turn turn = turn_of(p.slots, m0);
     if (!turn.mine) return;
+    // the channel this lane prepares and stores; lanes behind the last one stay for the shuffles, on the last one's values
+    const int64_t own = first + part % EACH;
+    const bool stores = part < EACH && own < p.channels;
     if (turn.slot < 0) {
-#pragma unroll
-        for (int k = 0; k < EACH; ++k)
-            if (c0 + k * CB < p.channels && part == 0)
-                store_one(static_cast<io_t *>(p.out.data), m0 * p.out.s0 + (c0 + k * CB) * p.out.s1, p.out.extent, 300, 0.0f);
+        if (stores) store_one(static_cast<io_t *>(p.out.data), m0 * p.out.s0 + own * p.out.s1, p.out.extent, 300, 0.0f);
         return;
     }
+    const int64_t co = own < p.channels ? own : p.channels - 1;
     const int64_t state_extent = p.slots.pool * p.channels * S;
-    // 4 states of B or C; lanes behind the last channel stay for the shuffles, on the last channel's values
-    const auto projection = [&](const View2 &v, int64_t m, int64_t g, int n, int have, int site, float (&f)[4]) {
-        const int64_t at = m * v.s0 + g * v.s1 + n * v.s2;
+    const float D = p.D != nullptr ? load_one(p.D, co, p.channels, 301) : 0.0f;
+    const float bias = p.dt_bias != nullptr ? load_one(p.dt_bias, co, p.channels, 302) : 0.0f;
+    const auto projection = [&](const View2 &v, int64_t at, int have, int site, float (&f)[4]) {
         if (p.vec_proj) {
             load_array(static_cast<const io_t *>(v.data), at, v.extent, site, f);
         } else {
@@ -124,42 +128,54 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const __grid_consta
             if (!turn.more) break;
             if (p.slots.slots[m] != turn.slot) continue;
         }
-        float x[EACH], dt[EACH], y[EACH], z[EACH];
-        int64_t cc[EACH];
+        const float x = load_one(static_cast<const io_t *>(p.x.data), m * p.x.s0 + co * p.x.s1, p.x.extent, 303);
+        float dt = load_one(static_cast<const io_t *>(p.dt.data), m * p.dt.s0 + co * p.dt.s1, p.dt.extent, 304);
+        const float z = p.z.data != nullptr ? load_one(static_cast<const io_t *>(p.z.data), m * p.z.s0 + co * p.z.s1, p.z.extent, 310) : 0.0f;
+        float y[EACH];
 #pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-            cc[k] = c0 + k * CB < p.channels ? c0 + k * CB : p.channels - 1;
-            x[k] = load_one(static_cast<const io_t *>(p.x.data), m * p.x.s0 + cc[k] * p.x.s1, p.x.extent, 303);
-            dt[k] = load_one(static_cast<const io_t *>(p.dt.data), m * p.dt.s0 + cc[k] * p.dt.s1, p.dt.extent, 304);
-            if (p.dt_bias != nullptr) dt[k] += load_one(p.dt_bias, cc[k], p.channels, 302);
-            z[k] = p.z.data != nullptr ? load_one(static_cast<const io_t *>(p.z.data), m * p.z.s0 + cc[k] * p.z.s1, p.z.extent, 310) : 0.0f;
-            y[k] = 0.0f;
-        }
-        for (int n = part * 4; n < S; n += LANES * 4) {
-            const int have = S - n < 4 ? S - n : 4;
-            float h[EACH][4], a[EACH][4], b[4], r[4];
+        for (int k = 0; k < EACH; ++k) y[k] = 0.0f;
+        bool prepared = false;
+        for (int n = part * 4; n - part * 4 < S; n += LANES * 4) {  // as often in all lanes
+            const int have = S - n < 4 ? S - n : 4;                // none: below 1
+            float h[EACH][4], a[EACH][4], b[4] = {}, r[4] = {};
 #pragma unroll
             for (int k = 0; k < EACH; ++k) {
-                quad(p.state, (turn.slot * p.channels + cc[k]) * S + n, have, state_extent, 305, h[k]);
-                quad(p.A, cc[k] * S + n, have, p.channels * S, 306, a[k]);
+                const int64_t c = first + k < p.channels ? first + k : p.channels - 1;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[k][i] = a[k][i] = 0.0f;
+                if (have > 0) {
+                    quad(p.state, (turn.slot * p.channels + c) * S + n, have, state_extent, 305, h[k]);
+                    quad(p.A, c * S + n, have, p.channels * S, 306, a[k]);
+                }
+            }
+            if (!prepared) {
+                dt += bias;
+                if (p.softplus) dt = softplus(dt);
+                prepared = true;
             }
             int64_t group = -1;
 #pragma unroll
             for (int k = 0; k < EACH; ++k) {
-                const int64_t g = p.per_group == p.channels ? 0 : cc[k] / p.per_group;
-                if (g != group) {
-                    projection(p.B, m, g, n, have, 307, b);
-                    projection(p.C, m, g, n, have, 308, r);
+                const int64_t c = first + k < p.channels ? first + k : p.channels - 1;
+                const int64_t g = p.per_group == p.channels ? 0 : c / p.per_group;
+                if (g != group && have > 0) {
+                    projection(p.B, m * p.B.s0 + g * p.B.s1 + n * p.B.s2, have, 307, b);
+                    projection(p.C, m * p.C.s0 + g * p.C.s1 + n * p.C.s2, have, 308, r);
                     group = g;
                 }
-                const float d = n == part * 4 ? (dt[k] = p.softplus ? softplus(dt[k]) : dt[k]) : dt[k], u = d * x[k];
+                float d = dt, v = x;
+                if constexpr (EACH > 1) {
+                    d = __shfl_sync(kFullMask, dt, k, 4);
+                    v = __shfl_sync(kFullMask, x, k, 4);
+                }
+                const float u = d * v, d2 = d * kLog2e;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    h[k][i] = fmaf(exp2_approx(d * (a[k][i] * kLog2e)), h[k][i], u * b[i]);
+                    h[k][i] = fmaf(exp2_approx(d2 * a[k][i]), h[k][i], u * b[i]);
                     if (i < have) y[k] = fmaf(r[i], h[k][i], y[k]);
                 }
-                if (c0 + k * CB < p.channels) {
-                    const int64_t at = (turn.slot * p.channels + cc[k]) * S + n;
+                if (first + k < p.channels && have > 0) {
+                    const int64_t at = (turn.slot * p.channels + c) * S + n;
                     if (p.vec) {
                         store_array(p.state, at, state_extent, 309, h[k]);
                     } else {
@@ -170,15 +186,11 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const __grid_consta
                 }
             }
         }
-#pragma unroll
-        for (int k = 0; k < EACH; ++k) {
-#pragma unroll
-            for (int d = LANES / 2; d >= 1; d >>= 1) y[k] += __shfl_xor_sync(kFullMask, y[k], d);
-            if (c0 + k * CB < p.channels && part == 0) {
-                if (p.D != nullptr) y[k] = fmaf(load_one(p.D, cc[k], p.channels, 301), x[k], y[k]);
-                if (p.z.data != nullptr) y[k] *= z[k] * logistic(z[k]);
-                store_one(static_cast<io_t *>(p.out.data), m * p.out.s0 + cc[k] * p.out.s1, p.out.extent, 300, y[k]);
-            }
+        float sum = sum_and_spread<LANES>(y, part);
+        if (stores) {
+            sum = fmaf(D, x, sum);
+            if (p.z.data != nullptr) sum *= z * logistic(z);
+            store_one(static_cast<io_t *>(p.out.data), m * p.out.s0 + own * p.out.s1, p.out.extent, 300, sum);
         }
     }
 }

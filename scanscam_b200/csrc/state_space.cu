@@ -562,14 +562,14 @@ int ssb_selective_step(const ssb_selective_step_t *p, void *stream) {
     a.state = p->state;
     return with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
-        // 4 channels a thread, their loads under way together, where that leaves the SMs two CTAs each
+        // 4 channels a thread where that leaves the SMs two CTAs each
         const auto launch = [&](auto lanes) {
-            constexpr int L = decltype(lanes)::value, CB = 128 / L;
-            const bool many = p->entries * ((p->channels + 4 * CB - 1) / (4 * CB)) >= 2 * sm_count();
-            const int64_t blocks = (p->channels + CB * (many ? 4 : 1) - 1) / (CB * (many ? 4 : 1));
+            constexpr int L = decltype(lanes)::value, CB = 128 / L, kEach = L >= 4 ? 4 : 1;
+            const bool many = p->entries * ((p->channels + kEach * CB - 1) / (kEach * CB)) >= 2 * sm_count();
+            const int64_t blocks = (p->channels + CB * (many ? kEach : 1) - 1) / (CB * (many ? kEach : 1));
             if (blocks > 65535) return fail(SSB_ERR_UNSUPPORTED, "too many channels");
             const dim3 grid((unsigned)p->entries, (unsigned)blocks);
-            if (many) ssb::selective_step_kernel<io_t, L, 4><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
+            if (many) ssb::selective_step_kernel<io_t, L, kEach><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
             else ssb::selective_step_kernel<io_t, L, 1><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
             return check_launch("selective_step_kernel");
         };
