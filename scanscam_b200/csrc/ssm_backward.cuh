@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
         const bool live = cl < channels;
         const int64_t c = c0 + (live ? cl : 0);
         const int have = live ? (S - ql * SPL < SPL ? S - ql * SPL : SPL) : 0;
-        pair_t A[2], dA[2] = {0, 0}, dA_before[2] = {0, 0};  // summed per tile, and over tiles: short chains of roundings
+        pair_t A[2], dA[2] = {0, 0};
         load_lane_decays<SPL>(p.A, c * S + ql * SPL, have, p.vec, p.channels * S, 261, A);
         for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
             const Span sp = span_of(p.seq, s);
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
                                 pair_t b[2];
                                 load_lane_projection<SPL>(Bs + t * H::SP, b);
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) h[e] = fma2(exp2_pair(mul2(dt2, A[e])), h[e], mul2(u2, b[e]));
+                                for (int e = 0; e < 2; ++e) h[e] = fma2(exp2_pair(fma2(dt2, A[e], both(kExponentShift))), h[e], mul2(u2, b[e]));
                             }
                             start[sub + 1][0] = h[0];
                             start[sub + 1][1] = h[1];
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
                                 pair_t sum;
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    a[i][e] = exp2_pair(mul2(dt2, A[e]));
+                                    a[i][e] = exp2_pair(fma2(dt2, A[e], both(kExponentShift)));
                                     m[i][e] = mul2(a[i][e], h[e]);  // a_t h_{t-1}
                                     h[e] = fma2(u2, b[i][e], m[i][e]);
                                     sum = e == 0 ? mul2(h[e], cc[i][e]) : fma2(h[e], cc[i][e], sum);
@@ -434,17 +434,12 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
                         }
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    dA_before[e] = add2(dA_before[e], dA[e]);
-                    dA[e] = 0;
-                }
                 __syncthreads();
             }
             if (q.gstate != nullptr) store_lane_states<SPL>(q.gstate, state_at, have, p.vec, state_extent, 243, adjoint);
         }
         store_lane_states<SPL>(q.part_A, ((int64_t)blockIdx.y * p.channels + c) * S + ql * SPL, have, p.vec,
-                               (int64_t)gridDim.y * p.channels * S, 244, dA_before);
+                               (int64_t)gridDim.y * p.channels * S, 244, dA);
     }
     __syncthreads();
     if (threadIdx.x < channels) {

@@ -83,6 +83,13 @@ __device__ __forceinline__ float sum_and_spread(float (&v)[STEPS], int q) {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
+// Added to the exponents of decays.  The unit's results lie 2e-8 of the value too low on average where decays are
+// slow (measured over [-0.1, -0.001]), which a state that remembers hundreds of steps adds up; a shift of the
+// exponent takes most of it back for the price of a multiply that becomes a multiply-add, and is lost in the
+// rounding of larger exponents, where nothing is remembered.  An exponent of zero still gives exactly 1.
+// [4, 2048, 2048]: error of the states 3e-7 with it, 5e-7 without; of the gradient of A 9e-7, 2e-6.
+constexpr float kExponentShift = 2e-8f;
+
 // 2^x on the special function unit: 8 cycles a warp instruction and sub-partition, error below
 // 1.5e-7 of the value (measured over [-100, 0]; a bias of at most 5e-8).
 __device__ __forceinline__ float exp2_approx(float x) {

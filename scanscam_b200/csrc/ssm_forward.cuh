@@ -438,7 +438,7 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_fwd_
                                 const pair_t dt2 = both(now.dx[i].x), u2 = both(now.dx[i].x * now.dx[i].y);
 #pragma unroll
                                 for (int e = 0; e < SPL / 2; ++e) {
-                                    h[e] = fma2(exp2_pair(mul2(dt2, A[e])), h[e], mul2(u2, now.b[i][e]));
+                                    h[e] = fma2(exp2_pair(fma2(dt2, A[e], both(kExponentShift))), h[e], mul2(u2, now.b[i][e]));
                                     sum = e == 0 ? mul2(h[e], now.r[i][e]) : fma2(h[e], now.r[i][e], sum);
                                 }
                                 const float2 f = halves(sum);

@@ -418,8 +418,8 @@ __global__ void __launch_bounds__(W * 32) selective_bwd_kernel(const __grid_cons
                         load8(Bs + n * H::PAD + tl * kRun, bv);
                         load8(Cs + n * H::PAD + tl * kRun, cv);
 #pragma unroll
-                        for (int k = 0; k < kRun; ++k) a[k] = exp2_pair(mul2(dt[k], A));
-                        pair_t P = exp2_pair(mul2(span, A)), F = mul2(u[0], both(bv[0]));  // P: the decay over all 8 steps
+                        for (int k = 0; k < kRun; ++k) a[k] = exp2_pair(fma2(dt[k], A, both(kExponentShift)));
+                        pair_t P = exp2_pair(fma2(span, A, both(kExponentShift))), F = mul2(u[0], both(bv[0]));  // P: the decay over all 8 steps
 #pragma unroll
                         for (int k = 1; k < kRun; ++k) F = fma2(u[k], both(bv[k]), mul2(a[k], F));
                         const pair_t P0 = P;

@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const __grid_consta
                 const float u = d * v, d2 = d * kLog2e;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    h[k][i] = fmaf(exp2_approx(d2 * a[k][i]), h[k][i], u * b[i]);
+                    h[k][i] = fmaf(exp2_approx(fmaf(d2, a[k][i], kExponentShift)), h[k][i], u * b[i]);
                     if (i < have) y[k] = fmaf(r[i], h[k][i], y[k]);
                 }
                 if (first + k < p.channels && have > 0) {

@@ -281,6 +281,18 @@ def test_scan_extreme_decays(layout):
     assert torch.equal(got["out"], want["out"])
 
 
+@pytest.mark.parametrize("n,c,s", [(1, 10, 16), (10, 500, 16), (1, 6, 100)])
+def test_scan_steps_of_zero_change_nothing(n, c, s):
+    """exp(0 A) is 1 to the last bit: the state comes out as it went in, its gradient too."""
+    o = make_scan(F32, "cl", n, c, 45, s, softplus=False, bias=False, state=True, seed=28)
+    o["dt"] = torch.zeros_like(o["dt"])
+    got, _, gstate = run_scan(o, False, back="state")
+    assert torch.equal(got["state"], o["state"]) and torch.equal(got["gstate"], gstate)
+    state = o["state"].clone()
+    sc.scan_selective_step(*(o[k][..., 0] if k != "A" else o[k] for k in ("x", "dt", "A", "B", "C")), state)
+    assert torch.equal(state, o["state"])
+
+
 def test_scan_extreme_step_logits():
     """softplus far from zero on both sides, and gates that are shut or wide open."""
     o = make_scan(F32, "rows", 1, 6, 32, 4, bias=False, seed=11, dt_scale=1e-3)
