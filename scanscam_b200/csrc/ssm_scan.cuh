@@ -1,6 +1,7 @@
-// Selective scan over whole sequences: per channel c and state n
+// Backward of the selective scan where channels are few or states more than 32 (else ssm_backward.cuh), with lanes
+// across time, and the sums over CTAs that both forms leave to it.  Per channel c and state n
 //     h_t = exp(dt_t A[c,n]) h_{t-1} + dt_t x_t B_t[n],     y_t = sum_n C_t[n] h_t + D x_t,     out = y silu(z),
-// and its backward, which runs the adjoint r_t = exp(dt_t A) (gy_t C_t + r_{t+1}) from the right.
+// whose backward runs the adjoint r_t = exp(dt_t A) (gy_t C_t + r_{t+1}) from the right.
 //
 // What bounds it: one exponential per (step, channel, state).  At 16 a clock and SM that is four
 // times what the tensors take to move in 16-bit storage, so the kernels are laid out around the
