@@ -101,13 +101,13 @@ __device__ __forceinline__ pair_t exp2_pair(pair_t x) {
     const float2 f = halves(x);
     return make_pair(exp2_approx(f.x), exp2_approx(f.y));
 }
-// e^x for |x| up to some tens without the error that rounding x * log2(e) would bring:
-// the product's rounding error and log2(e)'s own tail are put back as a factor 1 + lo * ln 2.
+// e^x without the error that rounding x * log2(e) would bring: the product's rounding error and log2(e)'s own
+// tail are put back as a factor 1 + lo * ln 2.  Infinite from 88.7 up, where the factor, which may lie below 1, is left out.
 __device__ __forceinline__ float exp_accurate(float x) {
     const float hi = x * kLog2e;
     const float lo = fmaf(x, 1.925963033500945e-8f, fmaf(x, kLog2e, -hi));
     const float e = exp2_approx(hi);
-    return isfinite(hi) ? fmaf(e, lo * kLn2, e) : e;
+    return isfinite(e) ? fmaf(e, lo * kLn2, e) : e;
 }
 __device__ __forceinline__ float reciprocal_approx(float x) {  // 0 for infinity; one unit in the last place
     float y;
