@@ -510,7 +510,7 @@ typedef struct ssb_short_conv {
     int dtype, silu, weight_f32;                  /* weight_f32: weight and bias are float32, else in `dtype` */
     int64_t batch, channels, steps, width;
     int64_t sequences;
-    const int32_t *offsets, *lengths;             /* offsets: channels-last views only (stride of c is 1) */
+    const int32_t *offsets, *lengths;             /* offsets: channels-last views only (stride of c is 1, or one channel) */
     ssb_view_t x, out;
     const void *weight, *bias;                    /* [C, W], [C] dense; bias optional */
     const void *state;                            /* the window carried in, oldest input first, or NULL for zero */

@@ -284,6 +284,9 @@ int check_width(int64_t width) {
     return width >= 2 && width <= 4 ? SSB_OK : fail(SSB_ERR_UNSUPPORTED, "width=%lld: 2, 3 and 4 are supported", (long long)width);
 }
 
+// Whether neighbouring channels are adjacent: always so of a single one, whose stride says nothing.
+bool adjacent_channels(const ssb_view_t &v, int64_t channels) { return channels == 1 || v.stride[1] == 1; }
+
 int check_conv(const ssb_short_conv_t *p, bool data) {
     if (p == nullptr) return fail(SSB_ERR_BAD_ARG, "NULL argument");
     if (int rc = check_sizes(p->dtype, {p->batch, p->channels, p->steps})) return rc;
@@ -292,7 +295,7 @@ int check_conv(const ssb_short_conv_t *p, bool data) {
     if (!data || p->channels == 0) return SSB_OK;
     if (p->batch > 0 && p->steps > 0) {
         if (int rc = check_data(p->x.data, p->dtype, "x")) return rc;
-        if (p->offsets != nullptr && p->x.stride[1] != 1)
+        if (p->offsets != nullptr && !adjacent_channels(p->x, p->channels))
             return fail(SSB_ERR_UNSUPPORTED, "packed sequences need a channels-last view of x");
     }
     if (int rc = check_data(p->weight, p->weight_f32 ? SSB_F32 : p->dtype, "weight")) return rc;
@@ -322,10 +325,10 @@ int conv_chunk(const ssb_short_conv_t *p) {
 ConvForm conv_form(const ssb_short_conv_t *p, std::initializer_list<const ssb_view_t *> views) {
     bool cl = true, vec = p->channels % 4 == 0;
     for (const ssb_view_t *v : views) {
-        cl = cl && v->stride[1] == 1;
+        // one channel of which time is adjacent is a row, but packed sequences need the channels-last kernels
+        cl = cl && (p->offsets != nullptr ? adjacent_channels(*v, p->channels) : v->stride[1] == 1);
         vec = vec && lumps(*v, p->dtype);
     }
-    // time adjacent as well (one channel, or one step): the rows kernels do as well, but packed rows need the others
     ConvForm f{cl, vec ? 4 : 1, 0, 0};
     const int64_t chunk = cl ? conv_chunk(p) * ssb::kConvWarps : 4 * 32 * ssb::kRun;
     f.channel_blocks = cl ? (p->channels + 32 * f.lump - 1) / (32 * f.lump) : (p->channels + ssb::kConvWarps - 1) / ssb::kConvWarps;
@@ -588,7 +591,7 @@ int ssb_short_conv_fwd(const ssb_short_conv_t *p, void *stream) {
     if (p->channels == 0 || count == 0) return SSB_OK;
     if (p->steps > 0)
         if (int rc = check_data(p->out.data, p->dtype, "out")) return rc;
-    if (p->offsets != nullptr && p->steps > 0 && p->out.stride[1] != 1)
+    if (p->offsets != nullptr && p->steps > 0 && !adjacent_channels(p->out, p->channels))
         return fail(SSB_ERR_UNSUPPORTED, "packed sequences need a channels-last view of out");
     ConvForm f = conv_form(p, {&p->x, &p->out});
     if (p->steps == 0) f = {true, 1, (p->channels + 31) / 32, 1};
@@ -620,7 +623,7 @@ int ssb_short_conv_bwd(const ssb_short_conv_t *p, const ssb_short_conv_grads_t *
     if (p->steps > 0 && p->batch > 0) {
         if (int rc = check_data(g->gout.data, p->dtype, "gout")) return rc;
         if (int rc = check_data(g->gx.data, p->dtype, "gx")) return rc;
-        if (p->offsets != nullptr && (g->gout.stride[1] != 1 || g->gx.stride[1] != 1))
+        if (p->offsets != nullptr && (!adjacent_channels(g->gout, p->channels) || !adjacent_channels(g->gx, p->channels)))
             return fail(SSB_ERR_UNSUPPORTED, "packed sequences need channels-last views");
     }
     const int weight_type = p->weight_f32 ? SSB_F32 : p->dtype;

@@ -1,11 +1,11 @@
-"""State-space operators on the GPU at the edges of what they take: step logits far from zero.
+"""State-space operators on the GPU at the edges of what they take: step logits far from zero, one channel.
 Definitions in 64 bits: tests/_state_space.py; tolerances: tests/test_state_space_gpu.py."""
 import pytest
 import torch
 
 import _state_space as ref
 import scanscam_b200 as sc
-from test_state_space_gpu import BF16, F16, F32, INF, make_scan, run_scan, scan_roundings
+from test_state_space_gpu import BF16, F16, F32, INF, check_conv, ints, make_conv, make_scan, run_scan, scan_roundings
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +36,23 @@ def test_scan_far_step_logits(n, c, s, dtype, layout):
     for k, v in got.items():
         kind = dtype if k in ("out", "gx", "gdt", "gz", "gB", "gC") else F32
         ref.check(v.reshape(want[k][0].shape), want[k], kind, base + channels + steps, k)
+
+
+# ---- one channel --------------------------------------------------------------------------------------
+@pytest.mark.parametrize("offsets,t", [([0, 1, 1, 3, 40, 40, 300], 300), ([2, 7], 9), ([0, 1], 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("layout", ["rows", "cl", "strided"])
+def test_conv_packed_single_channel(offsets, t, dtype, layout):
+    o = make_conv(dtype, layout, 1, 1, t, 4, state=True, count=len(offsets) - 1, seed=33)
+    check_conv(o, True, ref.spans_of(1, t, offsets=offsets), offsets=ints(offsets))
+
+
+@pytest.mark.parametrize("offsets", [None, [0, 5, 5, 64]])
+def test_scan_single_channel(offsets):
+    spans = ref.spans_of(1, 64, offsets=offsets)
+    for layout in ("rows", "cl"):
+        o = make_scan(F32, layout, 1, 1, 64, 16, state=True, count=len(spans), seed=34)
+        got, gout, gstate = run_scan(o, True, offsets=None if offsets is None else ints(offsets))
+        want = ref.scan_selective(**o, dt_softplus=True, spans=spans, gout=gout, gstate=gstate)
+        for k, v in got.items():
+            ref.check(v, want[k], F32, scan_roundings(o, True)[0] + 65, k)
