@@ -297,7 +297,9 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
         const bool live = cl < channels;
         const int64_t c = c0 + (live ? cl : 0);
         const int have = live ? (S - ql * SPL < SPL ? S - ql * SPL : SPL) : 0;
-        pair_t A[2], dA[2] = {0, 0};
+        pair_t A[2];
+        // the gradient of A: a tile's sum, and the sum over tiles.  One running sum would round thousands of terms against the whole.
+        pair_t dA[2] = {0, 0}, dA_tiles[2] = {0, 0};
         load_lane_decays<SPL>(p.A, c * S + ql * SPL, have, p.vec, p.channels * S, 261, A);
         for (int64_t s = blockIdx.y; s < p.seq.count; s += gridDim.y) {
             const Span sp = span_of(p.seq, s);
@@ -433,13 +435,18 @@ __global__ void __launch_bounds__(2 * WARPS * 32, 8 / WARPS) selective_lane_bwd_
                             }
                         }
                     }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        dA_tiles[e] = add2(dA_tiles[e], dA[e]);
+                        dA[e] = 0;
+                    }
                 }
                 __syncthreads();
             }
             if (q.gstate != nullptr) store_lane_states<SPL>(q.gstate, state_at, have, p.vec, state_extent, 243, adjoint);
         }
         store_lane_states<SPL>(q.part_A, ((int64_t)blockIdx.y * p.channels + c) * S + ql * SPL, have, p.vec,
-                               (int64_t)gridDim.y * p.channels * S, 244, dA);
+                               (int64_t)gridDim.y * p.channels * S, 244, dA_tiles);
     }
     __syncthreads();
     if (threadIdx.x < channels) {

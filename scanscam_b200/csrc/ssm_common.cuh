@@ -87,7 +87,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 // slow (measured over [-0.1, -0.001]), which a state that remembers hundreds of steps adds up; a shift of the
 // exponent takes most of it back for the price of a multiply that becomes a multiply-add, and is lost in the
 // rounding of larger exponents, where nothing is remembered.  An exponent of zero still gives exactly 1.
-// [4, 2048, 2048]: error of the states 3e-7 with it, 5e-7 without; of the gradient of A 9e-7, 2e-6.
+// [4, 2048, 2048], 16 states: error of the states 2.6e-7 of the norm with it, 5.0e-7 without.
 constexpr float kExponentShift = 2e-8f;
 
 // 2^x on the special function unit: 8 cycles a warp instruction and sub-partition, error below

@@ -1,4 +1,5 @@
-"""State-space operators on the GPU at the edges of what they take: step logits far from zero, one channel.
+"""State-space operators on the GPU at the edges of what they take: step logits far from zero, long
+sums, one channel.
 Definitions in 64 bits: tests/_state_space.py; tolerances: tests/test_state_space_gpu.py."""
 import pytest
 import torch
@@ -36,6 +37,24 @@ def test_scan_far_step_logits(n, c, s, dtype, layout):
     for k, v in got.items():
         kind = dtype if k in ("out", "gx", "gdt", "gz", "gB", "gC") else F32
         ref.check(v.reshape(want[k][0].shape), want[k], kind, base + channels + steps, k)
+
+
+def test_scan_gradient_of_decays_over_many_steps():
+    """8192 equal terms: added to one running sum each step rounds the same way, up to a quarter of 8192 roundings in all.
+
+    Sums of 32 steps, and of those over 256 tiles, are within 32 + 256.  A term is dt a h dh with a = exp(-1 .. -2): a is
+    off by 2.4 roundings and 12 of dt |A|, with a product and a sum 29 a step; h and dh are geometric sums with a ratio of at
+    most 0.37, 46 each; three products: 125 with a's own.  In all 413, of which 8192 / 4 would be five times as much."""
+    c, t, s = 4736, 8192, 16  # the form for many channels: c * s / 4 of at least 128 lanes an SM
+    ones = torch.ones(1, c, t, device="cuda")
+    A = -1 - torch.rand(c, s, generator=torch.Generator(device="cuda").manual_seed(32), device="cuda")
+    B = torch.ones(1, s, t, device="cuda")
+    A.requires_grad_(True)
+    (got,) = torch.autograd.grad(sc.scan_selective(ones, ones, A, B, B), A, ones)
+    some = slice(0, c, 148)  # a channel of every block of 32 and more
+    part = ones[:, some]
+    want = ref.scan_selective(part, part, A.detach()[some], B, B, spans=ref.spans_of(1, t), gout=part)
+    ref.check(got[some], want["gA"], F32, 413, "gA")
 
 
 # ---- one channel --------------------------------------------------------------------------------------
