@@ -20,7 +20,9 @@ from __future__ import annotations
 from typing import Any, Optional, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
+from torch.jit import is_tracing
 
 from . import cuda
 
@@ -28,7 +30,17 @@ Out = Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]
 
 
 def _wants_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _recorded() -> bool:
+    """Whether a call has to go through its autograd function although no gradient is asked for: a trace would keep
+    the allocation of the outputs alone, and a forward-mode derivative, which the functions refuse, would be dropped."""
+    return is_tracing() or forward_ad._current_level >= 0
 
 
 def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -52,7 +64,7 @@ class ScanSelective(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, x, dt, A, B, C, D, z, dt_bias, state, lengths, offsets, dt_softplus):
         out, state_out, checkpoints = cuda._ext().selective_forward(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths,
-                                                                    offsets, True)
+                                                                    offsets, any(ctx.needs_input_grad))
         ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, state, lengths, offsets, checkpoints)
         ctx.dt_softplus = dt_softplus
         ctx.set_materialize_grads(False)
@@ -96,11 +108,19 @@ def scan_selective(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     if C.dim() == 3:
         C = C.unsqueeze(1)
     A, D, dt_bias, state, lengths, offsets = map(_dense, (A, D, dt_bias, state, lengths, offsets))
-    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state) or _recorded():
         out, state_out = ScanSelective.apply(x, dt, A, B, C, D, z, dt_bias, state, lengths, offsets, dt_softplus)
     else:
         out, state_out, _ = cuda._ext().selective_forward(x, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, offsets, False)
     return (out, state_out) if return_state else out
+
+
+class ScanSelectiveStep(torch.autograd.Function):
+    """:func:`scan_selective_step` for traces; no gradient."""
+
+    @staticmethod
+    def forward(ctx: Any, x, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots):
+        return cuda._ext().selective_step(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus, slots)
 
 
 def scan_selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, state: torch.Tensor, *,
@@ -117,7 +137,8 @@ def scan_selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     :return: ``[M, C]``; carries no gradient (a call that would need one is refused)
     """
     _refuse_grad("scan_selective_step", x, dt, A, B, C, state, D, z, dt_bias)
-    return cuda._ext().selective_step(x, dt, _dense(A), B, C, state, _dense(D), z, _dense(dt_bias), dt_softplus, _dense(slots))
+    step = ScanSelectiveStep.apply if _recorded() else cuda._ext().selective_step
+    return step(x, dt, _dense(A), B, C, state, _dense(D), z, _dense(dt_bias), dt_softplus, _dense(slots))
 
 
 class ShortConv(torch.autograd.Function):
@@ -165,11 +186,19 @@ def short_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     weight, bias, state, lengths, offsets = map(_dense, (weight, bias, state, lengths, offsets))
     if offsets is not None and x.dim() == 3 and x.stride(1) != 1:
         x = x.mT.contiguous().mT
-    if _wants_grad(x, weight, bias, state):
+    if _wants_grad(x, weight, bias, state) or _recorded():
         out, state_out = ShortConv.apply(x, weight, bias, state, lengths, offsets, silu)
     else:
         out, state_out = cuda._ext().short_conv_forward(x, weight, bias, silu, state, lengths, offsets)
     return (out, state_out) if return_state else out
+
+
+class ShortConvStep(torch.autograd.Function):
+    """:func:`short_conv_step` for traces; no gradient."""
+
+    @staticmethod
+    def forward(ctx: Any, x, state, weight, bias, silu, slots):
+        return cuda._ext().short_conv_step(x, state, weight, bias, silu, slots)
 
 
 def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
@@ -183,4 +212,5 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     """
     silu = _silu(activation)
     _refuse_grad("short_conv_step", x, state, weight, bias)
-    return cuda._ext().short_conv_step(x, state, _dense(weight), _dense(bias), silu, _dense(slots))
+    step = ShortConvStep.apply if _recorded() else cuda._ext().short_conv_step
+    return step(x, state, _dense(weight), _dense(bias), silu, _dense(slots))

@@ -1,7 +1,94 @@
-"""State-space operators without a GPU: sizes of one."""
+"""State-space operators without a GPU: calls that no gradient is asked of, and sizes of one."""
 import ctypes
+import types
 
-from scanscam_b200 import _native
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import scanscam_b200
+from scanscam_b200 import _native, cuda
+
+
+# ---- forward-mode derivatives and traces ------------------------------------------------------------
+def fill(t: torch.Tensor, value: float) -> None:
+    """Writes as a kernel does, where neither autograd nor a trace sees it."""
+    at = (ctypes.c_float * t.numel()).from_address(t.data_ptr())
+    at[:] = [value] * t.numel()
+
+
+@pytest.fixture
+def stand_in(monkeypatch):
+    """An extension whose functions allocate, and fill with the sum of x, as the kernels would: no GPU is needed to
+    see what autograd and traces make of a call."""
+    calls = []
+
+    def made(x, *shapes):
+        calls.append(x)
+        total = sum((ctypes.c_float * x.numel()).from_address(x.data_ptr()))
+        outs = tuple(torch.empty(s) for s in shapes)
+        for out in outs:
+            fill(out, total)
+        return outs
+
+    ext = types.SimpleNamespace(
+        selective_forward=lambda x, dt, A, *rest: (*made(x, x.shape, (x.shape[0], *A.shape)), torch.empty(0)),
+        selective_step=lambda x, dt, A, B, C, state, *rest: made(x, x.shape)[0],
+        short_conv_forward=lambda x, w, *rest: made(x, x.shape, (x.shape[0], x.shape[1], w.shape[1] - 1)),
+        short_conv_step=lambda x, state, *rest: made(x, x.shape)[0])
+    monkeypatch.setattr(cuda, "_ext", lambda: ext)
+    return calls
+
+
+def call(name, x):
+    A, w = -torch.ones(6, 4), torch.ones(6, 4)
+    if name == "scan_selective":
+        return scanscam_b200.scan_selective(x, torch.ones(2, 6, 5), A, torch.ones(2, 4, 5), torch.ones(2, 4, 5))
+    if name == "short_conv":
+        return scanscam_b200.short_conv(x, w)
+    if name == "scan_selective_step":
+        return scanscam_b200.scan_selective_step(x, torch.ones(2, 6), A, torch.ones(2, 4), torch.ones(2, 4), torch.zeros(2, 6, 4))
+    return scanscam_b200.short_conv_step(x, torch.zeros(2, 6, 3), w)
+
+
+NAMES = ["scan_selective", "scan_selective_step", "short_conv", "short_conv_step"]
+
+
+def operand(name, value=1.0):
+    return torch.full((2, 6) if name.endswith("step") else (2, 6, 5), value)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_derivatives_are_refused(stand_in, name):
+    """They are not built: the call says so, as `scan` does, instead of giving a result without a tangent."""
+    x = operand(name)
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError):
+            call(name, forward_ad.make_dual(x, torch.ones_like(x)))
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            call(name, forward_ad.make_dual(x, torch.ones_like(x)))
+        assert forward_ad.unpack_dual(call(name, x)).tangent is None  # nothing to carry
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_a_trace_makes_the_call(stand_in, name, grad_mode):
+    """A trace of the call gives the values of its own inputs, not memory that was never written."""
+    with torch.set_grad_enabled(grad_mode):
+        traced = torch.jit.trace(lambda x: call(name, x), (operand(name),))
+        before = len(stand_in)
+        other = operand(name, 3.0)
+        out = traced(other)
+    assert len(stand_in) == before + 1
+    assert torch.equal(out, torch.full_like(other, float(other.sum())))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_ordinary_calls(stand_in, name):
+    for mode in (torch.no_grad, torch.enable_grad, torch.inference_mode):
+        with mode():
+            x = operand(name)
+            assert torch.equal(call(name, x), torch.full_like(x, float(x.sum())))
 
 
 # ---- one channel ----------------------------------------------------------------------------------------

@@ -1,12 +1,13 @@
 """State-space operators on the GPU at the edges of what they take: step logits far from zero, long
-sums, one channel.
+sums, one channel, traces.
 Definitions in 64 bits: tests/_state_space.py; tolerances: tests/test_state_space_gpu.py."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import _state_space as ref
 import scanscam_b200 as sc
-from test_state_space_gpu import BF16, F16, F32, INF, check_conv, ints, make_conv, make_scan, run_scan, scan_roundings
+from test_state_space_gpu import BF16, F16, F32, INF, check_conv, ints, make_conv, make_scan, randn, run_scan, scan_roundings
 
 pytestmark = pytest.mark.gpu
 
@@ -75,3 +76,32 @@ def test_scan_single_channel(offsets):
         want = ref.scan_selective(**o, dt_softplus=True, spans=spans, gout=gout, gstate=gstate)
         for k, v in got.items():
             ref.check(v, want[k], F32, scan_roundings(o, True)[0] + 65, k)
+
+
+# ---- traces and forward-mode derivatives ----------------------------------------------------------------
+def test_traced_calls_and_tangents():
+    o, v = make_scan(F32, "rows", 2, 6, 20, 4, seed=35), make_conv(F32, "rows", 2, 6, 20, 4, seed=36)
+    pos, kw = [o[k] for k in ("dt", "A", "B", "C")], {k: o[k] for k in ("D", "z", "dt_bias")}
+    states, windows = torch.zeros(2, 6, 4, device="cuda"), torch.zeros(2, 6, 3, device="cuda")
+    calls = [(lambda x: sc.scan_selective(x, *pos, **kw, dt_softplus=True), o["x"]), (lambda x: sc.short_conv(x, v["weight"], v["bias"]), v["x"]),
+             (lambda x: sc.scan_selective_step(x, o["dt"][..., 0], o["A"], o["B"][..., 0], o["C"][..., 0], states.zero_()), o["x"][..., 0]),
+             (lambda x: sc.short_conv_step(x, windows.zero_(), v["weight"]), v["x"][..., 0])]
+    with torch.no_grad():
+        for call, x in calls:
+            traced = torch.jit.trace(call, (torch.zeros_like(x),))
+            assert torch.equal(traced(x), call(x))
+            with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+                call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+def test_traced_calls_have_gradients():
+    """Traced without a gradient in sight, replayed with one: the call keeps what its backward needs."""
+    o = make_scan(F32, "rows", 2, 6, 40, 4, seed=37)
+    pos, gout = [o[k] for k in ("dt", "A", "B", "C")], randn(2, 6, 40, seed=38)
+    v = make_conv(F32, "rows", 2, 6, 40, 4, seed=39)
+    for call in (lambda x: sc.scan_selective(x, *pos, dt_softplus=True), lambda x: sc.short_conv(x, v["weight"], activation="silu")):
+        with torch.no_grad():
+            traced = torch.jit.trace(call, (torch.zeros_like(o["x"]),))
+        x = o["x"].clone().requires_grad_(True)
+        (got,), (want,) = (torch.autograd.grad(f(x), x, gout) for f in (traced, call))
+        assert torch.equal(got, want)
