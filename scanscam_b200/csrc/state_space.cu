@@ -551,7 +551,8 @@ int ssb_selective_step(const ssb_selective_step_t *p, void *stream) {
     a.vec = p->states % 4 == 0 && aligned(p->state, 16) && aligned(p->A, 16);
     a.vec_proj = p->states % 4 == 0;
     for (const ssb_view_t *v : {&p->B, &p->C})
-        a.vec_proj = a.vec_proj && aligned(v->data, 4 * size_of(p->dtype)) && v->stride[2] == 1 && v->stride[0] % 4 == 0 && v->stride[1] % 4 == 0;
+        a.vec_proj = a.vec_proj && aligned(v->data, 4 * size_of(p->dtype)) && v->stride[2] == 1 && v->stride[0] % 4 == 0 &&
+                     (p->groups == 1 || v->stride[1] % 4 == 0);  // of one group the stride says nothing
     a.slots = {p->slots, p->entries, p->pool};
     a.x = view2(p->x, p->entries, p->channels);
     a.dt = view2(p->dt, p->entries, p->channels);

@@ -1,5 +1,5 @@
 """State-space operators on the GPU at the edges of what they take: step logits far from zero, long
-sums, one channel, traces.
+sums, one channel, projections of one group, traces.
 Definitions in 64 bits: tests/_state_space.py; tolerances: tests/test_state_space_gpu.py."""
 import pytest
 import torch
@@ -76,6 +76,19 @@ def test_scan_single_channel(offsets):
         want = ref.scan_selective(**o, dt_softplus=True, spans=spans, gout=gout, gstate=gstate)
         for k, v in got.items():
             ref.check(v, want[k], F32, scan_roundings(o, True)[0] + 65, k)
+
+
+# ---- projections of one group ---------------------------------------------------------------------------
+@pytest.mark.parametrize("m,c,s", [(3, 40, 16), (64, 1024, 16), (5, 33, 7)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_step_two_dimensional_projections(m, c, s, dtype):
+    """[M, S], dense or a slice at an odd place of a projection, is [M, 1, S]."""
+    x, dt, A = randn(m, c, seed=1, dtype=dtype), randn(m, c, seed=2, dtype=dtype), -torch.exp(randn(c, s, seed=3))
+    wide = randn(m, 3 * s, seed=4, dtype=dtype)
+    for B, C in ((wide[:, :s].contiguous(), wide[:, s: 2 * s].contiguous()), (wide[:, 1: s + 1], wide[:, 2 * s:])):
+        states = [randn(m, c, s, seed=5) for _ in range(2)]
+        outs = [sc.scan_selective_step(x, dt, A, b, r, state, dt_softplus=True) for b, r, state in ((B, C, states[0]), (B[:, None], C[:, None], states[1]))]
+        assert torch.equal(*outs) and torch.equal(*states)
 
 
 # ---- traces and forward-mode derivatives ----------------------------------------------------------------
