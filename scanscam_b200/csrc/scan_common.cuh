@@ -45,8 +45,6 @@ __device__ __forceinline__ bool index_in_range(int64_t index, int64_t extent, in
     return false;
 }
 #define SSB_INDEX_OK(index, extent, site) ::ssb::index_in_range((int64_t)(index), (int64_t)(extent), (site))
-// Submits one index to the test without touching memory (the self-test of the reporting path).
-__global__ void index_check_probe_kernel(int64_t index, int64_t extent) { (void)SSB_INDEX_OK(index, extent, 99); }
 #else
 #define SSB_INDEX_OK(index, extent, site) true
 #endif

@@ -2163,6 +2163,11 @@ int shard_map_publish(const float *gate, const float *in1, int64_t rows, int64_t
                                         T / 4, cut, nullptr, walked, px, (int)(epoch & 1u), epoch);
     return check_launch("tail_map_kernel<publish>");
 }
+
+#ifdef SSB_CHECKED
+// Submits one index to the test without touching memory (the self-test of the reporting path).
+__global__ void index_check_probe_kernel(int64_t index, int64_t extent) { (void)SSB_INDEX_OK(index, extent, 99); }
+#endif
 }  // namespace
 
 extern "C" {
@@ -2273,7 +2278,7 @@ int ssb_checked_build(void) {
 
 int ssb_selftest_index_check(void *stream) {
 #ifdef SSB_CHECKED
-    ssb::index_check_probe_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(5, 4);
+    index_check_probe_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(5, 4);
     return check_launch("index_check_probe_kernel");
 #else
     (void)stream;

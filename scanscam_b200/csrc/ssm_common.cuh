@@ -2,11 +2,7 @@
 // channels in one 64-bit register, and the three functions (2^x, softplus, logistic) they use.
 #pragma once
 
-// The checked build's self-test kernel is defined in that header, for the other translation unit;
-// here it goes by another name, so that the two link.
-#define index_check_probe_kernel state_space_index_probe_kernel
 #include "scan_common.cuh"
-#undef index_check_probe_kernel
 
 namespace ssb {
 
