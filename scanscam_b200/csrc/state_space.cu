@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <limits>
 
 #include "host_common.h"
@@ -101,15 +102,16 @@ int allow_smem(K kernel, size_t bytes) {
     return e == cudaSuccess ? SSB_OK : fail(SSB_ERR_LAUNCH, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
 }
 
-// A kernel whose warps pass registers to one another has to be launched with as many as they will hold in all,
-// or those that ask for more wait for good.
+// Registers of a thread of a kernel, as built; -1 where no device answers.
 template <auto kKernel>
-int check_registers() {
-    static const int registers = [] {
+int registers_of() {
+    static std::atomic<int> known{-1};
+    if (known < 0) {
         cudaFuncAttributes a;
-        return cudaFuncGetAttributes(&a, kKernel) == cudaSuccess ? a.numRegs : -1;
-    }();
-    return registers == ssb::kLaunchRegisters ? SSB_OK : fail(SSB_ERR_LAUNCH, "kernel built with %d registers, not %d", registers, ssb::kLaunchRegisters);
+        if (cudaFuncGetAttributes(&a, kKernel) == cudaSuccess) known = a.numRegs;
+        else (void)cudaGetLastError();
+    }
+    return known;
 }
 
 // ---- selective scan -----------------------------------------------------------------------------
@@ -188,10 +190,35 @@ int check_selective(const ssb_selective_t *p, bool data) {
 
 int64_t count_of(const ssb_selective_t *p) { return p->offsets != nullptr ? p->sequences : p->batch; }
 
+// Calls f with the lanes that share a channel in the backward with lanes across states.
+template <typename F>
+int with_backward_lanes(int64_t states, F &&f) {
+    if (states <= 8) return f(std::integral_constant<int, 2>{});
+    if (states <= 16) return f(std::integral_constant<int, 4>{});
+    return f(std::integral_constant<int, 8>{});
+}
+
+// That form's warps pass registers to one another: its kernel has to be launched with as many as they will hold in
+// all, or those that ask for more wait for good.  How many it was built with is the compiler's doing.
+template <auto kKernel>
+bool registers_fit() {
+    const int registers = registers_of<kKernel>();
+    return registers < 0 || registers == ssb::kLaunchRegisters;
+}
+bool lane_backward_fits(const ssb_selective_t *p) {
+    return with_type(p->dtype, [&](auto *type) {
+        using io_t = std::remove_pointer_t<decltype(type)>;
+        return with_backward_lanes(p->states, [](auto lanes) {
+            return (int)registers_fit<ssb::selective_lane_bwd_kernel<io_t, decltype(lanes)::value, kLaneWarps>>();
+        });
+    });
+}
+
 // The backward's shape.  Up to 32 states and with a warp for most schedulers: lanes across states
 // (ssm_backward.cuh; [4, 2048, 2048], 16 states: 469 us against 699).  The sums of B and C that its warps keep in
 // shared memory grow with the states, and a warp walks all steps of its sequence, so else lanes across time
 // (ssm_scan.cuh; [2, 1024, 1024], 64 states: 423 us against 703; [2, 387, 1001], 10 states: 106 us against 166).
+// The forward asks as well: the steps between its checkpoints depend on the answer.
 struct BackwardForm {
     bool lanes;
     int split;             // lanes across time of the other form
@@ -199,7 +226,8 @@ struct BackwardForm {
 };
 BackwardForm backward_form(const ssb_selective_t *p) {
     const int64_t per_group = p->channels / p->groups;
-    if (p->states <= kLaneBackwardStates && p->channels * count_of(p) * ((p->states + 3) / 4) >= 4 * 32 * (int64_t)sm_count()) {
+    if (p->states <= kLaneBackwardStates && p->channels * count_of(p) * ((p->states + 3) / 4) >= 4 * 32 * (int64_t)sm_count() &&
+        lane_backward_fits(p)) {
         const int64_t cb = kLaneWarps * 32 / (p->states <= 8 ? 2 : p->states <= 16 ? 4 : 8);
         return {true, 0, ssb::kCheckpointSteps, (per_group + cb - 1) / cb};
     }
@@ -465,7 +493,7 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
     const int rc = with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
         if (form.lanes) {
-            const auto launch = [&](auto lanes) {
+            return with_backward_lanes(p->states, [&](auto lanes) {
                 constexpr int LN = decltype(lanes)::value;
                 using H = ssb::LaneShape<LN, 4, kLaneWarps>;
                 ssb::SelectiveArgs a = selective_args(p, form.blocks);
@@ -477,15 +505,12 @@ int ssb_selective_bwd(const ssb_selective_t *p, const ssb_selective_grads_t *g, 
                 auto kernel = ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>;
                 constexpr size_t smem = ssb::selective_lane_bwd_smem<io_t, LN, kLaneWarps>();
                 if (int bad = allow_smem(kernel, smem)) return bad;
-                if (int bad = check_registers<ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>>()) return bad;
+                if (registers_of<ssb::selective_lane_bwd_kernel<io_t, LN, kLaneWarps>>() != ssb::kLaunchRegisters)
+                    return fail(SSB_ERR_LAUNCH, "the registers of selective_lane_bwd_kernel are not known");
                 const dim3 grid((unsigned)(form.blocks * p->groups), (unsigned)parts.parts_seq);
                 kernel<<<grid, 2 * H::THREADS, smem, (cudaStream_t)stream>>>(a, b);
                 return check_launch("selective_lane_bwd_kernel");
-            };
-            using std::integral_constant;
-            if (p->states <= 8) return launch(integral_constant<int, 2>{});
-            if (p->states <= 16) return launch(integral_constant<int, 4>{});
-            return launch(integral_constant<int, 8>{});
+            });
         }
         return with_split(form.split, [&](auto k) {
             constexpr int TL = decltype(k)::value;

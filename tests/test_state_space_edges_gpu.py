@@ -1,12 +1,15 @@
 """State-space operators on the GPU at the edges of what they take: step logits far from zero, long
 sums, one channel, projections of one group, traces.
 Definitions in 64 bits: tests/_state_space.py; tolerances: tests/test_state_space_gpu.py."""
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import _state_space as ref
 import scanscam_b200 as sc
+from scanscam_b200 import _native
 from test_state_space_gpu import BF16, F16, F32, INF, check_conv, ints, make_conv, make_scan, randn, run_scan, scan_roundings
 
 pytestmark = pytest.mark.gpu
@@ -56,6 +59,16 @@ def test_scan_gradient_of_decays_over_many_steps():
     part = ones[:, some]
     want = ref.scan_selective(part, part, A.detach()[some], B, B, spans=ref.spans_of(1, t), gout=part)
     ref.check(got[some], want["gA"], F32, 413, "gA")
+
+
+@pytest.mark.parametrize("dtype", ["F32", "BF16", "F16"])
+@pytest.mark.parametrize("states", [8, 16, 32])
+def test_scan_form_for_many_channels_is_built(native, dtype, states):
+    """Its kernels pass registers between warps and need the compiler to give them a certain number.  Where it did not, the
+    other form does the work, slower: its checkpoints lie 32 steps apart at least, this one's 16."""
+    n, c, t = 4, 5000, 100
+    p = _native.Selective(dtype=getattr(_native, dtype), batch=n, channels=c, steps=t, states=states, groups=1)
+    assert native.ssb_selective_checkpoint_bytes(ctypes.byref(p)) == n * -(-t // 16) * c * states * 4
 
 
 # ---- one channel --------------------------------------------------------------------------------------
