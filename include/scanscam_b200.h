@@ -453,8 +453,9 @@ int ssb_shard_carry_peer_f32(const ssb_peer_exchange_t *exchange, unsigned epoch
  * projection and either layout (time adjacent, or channels adjacent) are taken as they are.
  * Sequences: row n of the batch is sequence n, all `steps` of it or its first lengths[n]; or, with
  * `offsets` (batch must be 1), sequence s is steps offsets[s] .. offsets[s+1] of the one row.
- * offsets and lengths are read on the device and cut to [0, steps].  Outputs and gradients at
- * steps that no sequence covers are zero.  Per-sequence states are dense: [sequences, C, S] float32
+ * offsets, which must not fall, and lengths are read on the device and cut to [0, steps].  Outputs and
+ * gradients at steps that no sequence covers are zero.  Outputs must not overlap inputs: a carried-in
+ * state is read while the carried-out one is written.  Per-sequence states are dense: [sequences, C, S] float32
  * for the scan, [sequences, C, W-1] in the tensors' type for the convolution.
  * All arithmetic, states and sums are float32; an output is rounded once.
  * ---------------------------------------------------------------------------------- */

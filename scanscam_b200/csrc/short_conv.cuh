@@ -2,10 +2,13 @@
 // widths 2, 3 and 4, and its backward.  What lies before a sequence's first step is the window
 // carried in (the last W-1 inputs of the piece before, oldest first), or zero.
 //
-// Memory-bound: 2 tensors forward, 3 more backward.  Two forms:
+// The floor: 2 tensors forward, 3 more backward.  Channels last, [8, 4096, 2048] in bf16 with 4 taps: 73 us forward (41 for the bytes), where
+// 14 warps an SM wait for their loads, and 141 backward (61), where instructions count (160 a warp for 4 channels and a step).
+// Two forms:
 //   channels last   a thread owns V adjacent channels (one 8- or 16-byte access per step) and walks
 //                   a chunk of steps with its window in registers; the steps before its chunk are read again;
-//   rows            a warp owns a row; a lane takes 8 adjacent steps and reads its neighbours' few from cache.
+//   rows            a warp owns a row; a lane takes 8 adjacent steps, element by element, and reads its neighbours' few from cache
+//                   ([3, 515, 1001] fp32, 3 taps: 14 + 20 us, 1.9 + 2.8 for the bytes).
 #pragma once
 
 #include "ssm_common.cuh"

@@ -1,20 +1,22 @@
 // Selective scan over whole sequences, forward: per channel c and state n
 //     h_t = exp(dt_t A[c,n]) h_{t-1} + dt_t x_t B_t[n],     y_t = sum_n C_t[n] h_t + D x_t,     out = y silu(z).
 //
-// What bounds it: one exponential per (step, channel, state).  At 16 a clock and SM they take three
-// times as long as the tensors' bytes in 16-bit storage, so the states never leave the registers and
-// everything else is kept below 8 issue slots an exponential.
+// The floor: one exponential per (step, channel, state).  At 16 a clock and SM they take three times as long as the
+// tensors' bytes in 16-bit storage, so the states stay in registers (but for the checkpoints of a training call).
+// What bounds it: everything else takes 9.9 instructions an exponential with 8 states a lane, 12.6 with 4 and 13.5
+// where checkpoints are written, in all warps together; and with few channels a warp waits out each step alone.
 //
-// LN lanes share a channel, each with SPL of its states (4; 8 beyond 128 states); a warp holds
-// 32 / LN channels and walks the steps in order.  Per step and 4 states a lane issues 4 exponentials,
+// LN lanes share a channel, each with SPL of its states (4; 8 where warps abound, and beyond 128 states); a warp
+// holds 32 / LN channels and walks the steps in order.  Per step and 4 states a lane issues 4 exponentials,
 // 8 packed operations (exponent, input, recurrence, read-out, two states each) and 3 shared loads.
 // The read-out is summed over the LN lanes for groups of steps, so that each lane is left with the sum
-// of one step (LN = 4: 3 shuffles for 4 steps).  A tile of 32 steps is put into shared memory by the whole CTA: (dt, x)
-// after the softplus, B and C as fp32; the next tile's bytes are fetched meanwhile.  The sums take the
-// place of the steps in shared memory and leave, gated, with 16-byte stores.
+// of one step (LN = 4: 3 shuffles for 4 steps).  Half of the CTA's warps scan; the other half put tiles of 32
+// steps into shared memory, (dt, x) after the softplus, B and C as fp32, and fetch the next tile's bytes meanwhile.  The
+// sums take the place of the steps in shared memory, from where those warps send them, gated: 16 bytes at a time where
+// all operands allow it.
 //
 // Measured, bf16, 16 states: 13 packed prompts in [1, 4096, 4096] 136 us with 8 states a lane (169 with 4); [4, 2048, 2048]
-// 183 us; [1, 2048, 8192] 505 us, where a scheduler has one scanning warp and a step's latency (119 cycles) counts.
+// 183 us; [1, 2048, 8192] 505 us, where a scheduler has one scanning warp and a step's latency (121 cycles at 1.965 GHz) counts.
 // The exponentials alone are 58 us in each.
 #pragma once
 

@@ -3,10 +3,13 @@
 //     h_t = exp(dt_t A[c,n]) h_{t-1} + dt_t x_t B_t[n],     y_t = sum_n C_t[n] h_t + D x_t,     out = y silu(z),
 // whose backward runs the adjoint r_t = exp(dt_t A) (gy_t C_t + r_{t+1}) from the right.
 //
-// What bounds it: one exponential per (step, channel, state).  At 16 a clock and SM that is four
-// times what the tensors take to move in 16-bit storage, so the kernels are laid out around the
-// arithmetic: the states are never written to memory, and the recurrence is cut along time inside
-// the warp so that an exponential is computed once and used twice (fold and replay).
+// The forward writes one state in a tile of steps; the others are rebuilt here.  The recurrence is cut along time inside
+// the warp so that an exponential is computed once and used in both directions (fold and replay), with one more for the
+// decay over a thread's 8 steps: 9/8 a (step, channel, state).
+//
+// What bounds it: latency.  254 registers leave 8 warps an SM, and a turn over a state composes two maps by dependent
+// shuffles and ends in a barrier.  [2, 1024, 1024], 64 states in 4 groups, fp16: 422 us, 40 instructions an exponential in
+// 37 % of the issue slots, against 29 us for the exponentials alone.
 //
 // A thread holds 8 consecutive steps of 2 adjacent channels (pairs in 64-bit registers) and goes
 // through the states one by one.  For a state it folds its 8 steps to an affine map, the TL lanes
@@ -298,8 +301,7 @@ struct ScanShape {
 // ---- backward -----------------------------------------------------------------------------------
 // Tiles run from the last to the first.  Each starts from its checkpoint (the state the forward
 // wrote at the tile's first step), rebuilds the states as the forward does, and carries the adjoint
-// r to the tile on its left.  Per (step, channel, state) there is one exponential and 17 fp32
-// operations, so the fp32 pipe bounds it, not the special function unit.
+// r to the tile on its left.  Per (step, channel, state) there are 9/8 exponentials and 17 fp32 operations.
 //
 // The gradients of B and C sum over channels: over the pair in the thread, over the DL lanes by an
 // exchange that halves the number of values at each step (16 values: 8 + 4 shuffles for DL = 4),

@@ -6,8 +6,10 @@
 // sequence, in the order of the batch: the first of them computes them all, so that no two CTAs
 // ever work on one state and the result does not depend on their timing.
 //
-// Bound by the state pool's rows, read and written once (4-byte states: 8 S bytes per channel), and
-// for few entries by the launch.
+// The floor: the state pool's rows, read and written once (4-byte states: 8 S bytes per channel); for few entries the
+// launch.  256 entries, bf16: scan of 4096 channels with 16 states 48 us (22 for the bytes), convolution of 8192 channels 9.3
+// (5.1).  What is between: the slot, the list of slots and the state are asked for one after the other, and every CTA
+// reads the whole list: 8192 entries of 1024 channels take 379 us without slots and 678 with them, the convolution 25 and 126.
 #pragma once
 
 #include "ssm_common.cuh"

@@ -1,5 +1,5 @@
 // C-ABI entry points of the state-space operators: argument checks, choice of the kernel's shape,
-// launches.  Kernels: ssm_scan.cuh, ssm_step.cuh, short_conv.cuh.
+// launches.  Kernels: ssm_forward.cuh, ssm_backward.cuh, ssm_scan.cuh, ssm_step.cuh, short_conv.cuh.
 #include "../../include/scanscam_b200.h"
 
 #include <cuda_runtime.h>
@@ -432,7 +432,7 @@ int ssb_selective_fwd(const ssb_selective_t *p, void *stream) {
     return with_type(p->dtype, [&](auto *type) {
         using io_t = std::remove_pointer_t<decltype(type)>;
         const int64_t per_group = p->channels / p->groups;
-        // 8 states a lane need 5 instructions an exponential where 4 need 8, but a warp alone on its scheduler takes
+        // 8 states a lane need 9.9 instructions an exponential where 4 need 12.6, but a warp alone on its scheduler takes
         // as long for either: from two warps a scheduler up (13 prompts of 4096 channels, 16 states: 136 us against
         // 169; [4, 2048, 2048], half a warp a scheduler: 179 against 177; [1, 2048, 8192]: 636 against 505).
         const bool eight = p->channels * count * ((p->states + 7) / 8) >= 2 * 4 * 32 * (int64_t)sm_count();

@@ -7,7 +7,8 @@ would be ``[N, C, S, T]`` tensors, ``S`` times what goes in and out.  Here they 
 
 Layouts are the package's: ``[N, C, T]`` with time last, dense or as the ``[N, C, T]`` view of dense
 ``[N, T, C]`` (channels last), or any slice of a larger tensor; outputs and gradients have the
-layout (channels adjacent or steps adjacent) of the operand they belong to.  float32, bfloat16 and
+layout (channels adjacent or steps adjacent) of the operand they belong to, but a packed convolution gives channels last.
+Fastest are operands of one layout whose rows start on 16 bytes; others are fetched element by element.  float32, bfloat16 and
 float16 tensors are taken; the arithmetic, the states and all sums are float32.
 
 A batch holds one sequence per row, of all ``T`` steps or of the first ``lengths[n]``; or it is one
