@@ -51,6 +51,8 @@ def _dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 def _refuse_grad(name: str, *tensors: Optional[torch.Tensor]) -> None:
     if _wants_grad(*tensors):
         raise RuntimeError(f"scanscam_b200.{name} updates its state in place and has no gradient; call it under torch.no_grad()")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"scanscam_b200.{name} has no forward-mode derivative")
 
 
 def _silu(activation: Optional[str]) -> bool:
@@ -138,7 +140,7 @@ def scan_selective_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
     :return: ``[M, C]``; carries no gradient (a call that would need one is refused)
     """
     _refuse_grad("scan_selective_step", x, dt, A, B, C, state, D, z, dt_bias)
-    step = ScanSelectiveStep.apply if _recorded() else cuda._ext().selective_step
+    step = ScanSelectiveStep.apply if is_tracing() else cuda._ext().selective_step
     return step(x, dt, _dense(A), B, C, state, _dense(D), z, _dense(dt_bias), dt_softplus, _dense(slots))
 
 
@@ -213,5 +215,5 @@ def short_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, 
     """
     silu = _silu(activation)
     _refuse_grad("short_conv_step", x, state, weight, bias)
-    step = ShortConvStep.apply if _recorded() else cuda._ext().short_conv_step
+    step = ShortConvStep.apply if is_tracing() else cuda._ext().short_conv_step
     return step(x, state, _dense(weight), _dense(bias), silu, _dense(slots))

@@ -70,6 +70,18 @@ def test_forward_mode_derivatives_are_refused(stand_in, name):
         assert forward_ad.unpack_dual(call(name, x)).tangent is None  # nothing to carry
 
 
+@pytest.mark.parametrize("name", ["scan_selective_step", "short_conv_step"])
+def test_a_refused_step_leaves_its_state(stand_in, name):
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(operand(name), torch.ones(2, 6))
+        with pytest.raises(NotImplementedError):
+            call(name, dual)
+        # the same where the tangent comes with another operand
+        with pytest.raises(NotImplementedError):
+            scanscam_b200.short_conv_step(operand(name), torch.zeros(2, 6, 3), forward_ad.make_dual(torch.ones(6, 4), torch.ones(6, 4)))
+    assert not stand_in  # no kernel ran
+
+
 @pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("grad_mode", [True, False])
 def test_a_trace_makes_the_call(stand_in, name, grad_mode):
